@@ -40,8 +40,11 @@ def build(force=False, verbose=True, tuning=False):
         return out
     objdir = os.path.join(HERE, "build", "tuning" if tuning else "product")
     os.makedirs(objdir, exist_ok=True)
-    # kernel-argument preload: the first 16 dwords of a kernel's scalar arguments arrive in SGPRs with the wave
+    # kernel-argument preload: the first 16 dwords of a kernel's scalar arguments arrive in SGPRs with the wave.
+    # packed fp32 arithmetic off: some forms of v_pk_*_f32 that the compiler makes from ordinary float code have given
+    # wrong results on these cards now and then (the host pass does not know the feature and says so: harmless)
     flags = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-mllvm", "-amdgpu-kernarg-preload-count=16",
+             "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-I", os.path.join(ROOT, "include"), "-I", HERE] + (["-DQTTS_TUNING"] if tuning else [])
 
     def compile_unit(src):
