@@ -101,6 +101,40 @@ int qtts_linear_swiglu_fp8(const void *x, int ldx, const void *w_gate_up_fp8_pac
                            const float *w_scales, const void *norm_w, float eps, void *out,
                            int ldo, int M, int I, int K, qtts_stream_t stream);
 
+/* ---- 8-bit integers (W8A8): an extension, the reference has bf16 only.  Activation rows and weight rows are int8 with one
+ * fp32 scale each, a row standing for q * scale.  A product's integer sum is exact (int32, K <= 131071); what follows it is
+ * fp32 with ONE rounding, to bf16, at the store.  int8 activations are [M, ld] with ld % 16 == 0, 16-byte aligned: the bytes
+ * K .. round_up(K, 16) of every row (the last one included) must be readable, whatever they hold, and are never written.
+ * M, N, I >= 1 and K, H >= 1 are free of multiples.  bf16 rows of any stride and 2-byte alignment are taken; 16-byte
+ * aligned ones (strides % 8) are faster.  A row that holds a NaN or an infinity gets a scale that is NaN or infinite and
+ * q = 0: everything computed from that row is NaN, no other row is touched.
+ *
+ * qtts_quantize_int8: scales[m] = max(max|x[m]| / 127, 2^-126), q[m] = rint(x[m] / scales[m]), |q| <= 127.
+ * (Also quantises F.linear weights [N,K] per output channel, for qtts_pack_weight_int8.)
+ * qtts_rmsnorm_int8: h = bf16(x + delta) is written to `sum` (which may be x or delta itself, with its stride); then
+ * y = h / sqrt(mean(h^2) + eps) * w in fp32, not rounded in between, quantised as above.  delta == sum == NULL: h = x.
+ * The norm of P/layers/layernorm.py:17-27 behind the residual addition of P/models/qwen3_tts_share.py:171,175. */
+int qtts_quantize_int8(const void *x, int ldx, void *q, int ldq, float *scales, int M, int K, qtts_stream_t stream);
+int qtts_rmsnorm_int8(const void *x, int ldx, const void *delta, int ldd, const void *w, float eps, void *sum, int lds,
+                      void *q, int ldq, float *scales, int M, int H, qtts_stream_t stream);
+/* int8 rows [N, ldw] (any stride >= K, any alignment) -> fragment order [ceil(N/16)][2 ceil(K/128)][64 lanes][16 B], lane
+ * (g, r) = row 16 * tile + r, columns 64 * step + 16 g .. +16; zeros behind the last row and column.  gate_up: tile t holds
+ * outputs 8t .. 8t+7, its row 4p + j the gate row (j < 2) or the up row (j >= 2) of output 8t + 2p + j % 2. */
+size_t qtts_packed_weight_int8_bytes(int N, int K);
+size_t qtts_packed_gate_up_int8_bytes(int I, int K);
+int qtts_pack_weight_int8(const void *w, int ldw, void *packed, int N, int K, qtts_stream_t stream);
+int qtts_pack_gate_up_int8(const void *gate, const void *up, int ldw, void *packed, int I, int K, qtts_stream_t stream);
+/* out[m,n] = bf16(x_scales[m] * w_scales[n] * sum_k x[m,k] w[n,k] + bias[n] + residual[m,n]); bias and residual may be NULL,
+ * out may be the residual itself (same stride). */
+int qtts_linear_int8(const void *x, int ldx, const float *x_scales, const void *w_packed, const float *w_scales,
+                     const void *bias, const void *residual, int ldr, void *out, int ldo, int M, int N, int K,
+                     qtts_stream_t stream);
+/* out[m,i] = bf16(silu(g) * u), g and u the scaled sums with gate row i and up row i (gate_scales / up_scales [I], in the
+ * rows' own order).  P/models/qwen3_tts_share.py:131-135 without its bf16 roundings of g, u and silu(g). */
+int qtts_linear_swiglu_int8(const void *x, int ldx, const float *x_scales, const void *w_gate_up_packed,
+                            const float *gate_scales, const float *up_scales, void *out, int ldo, int M, int I, int K,
+                            qtts_stream_t stream);
+
 /* out[M,I] = silu(x@Wg^T) * (x@Wu^T) with the reference's two roundings
  * (P/models/qwen3_tts_share.py:131-135, P/layers/activation.py:11-13);
  * optional fused RMSNorm of x as above. */

@@ -2,9 +2,9 @@
 
     python nano-qwen3tts-vllm_amd/csrc/build.py [--force] [--tuning]
 
-The library is four translation units over one shared header (qtts_common.h): qtts_gemm.hip (weight packing, the decode
-and prompt GEMM kernels, RMSNorm), qtts_attention.hip, qtts_glue.hip (picks, gathers, per-frame glue) and qtts_model.hip
-(the decoder stack, graphs).  They are compiled side by side and linked into one shared object.
+The library is five translation units over one shared header (qtts_common.h): qtts_gemm.hip (weight packing, the decode
+and prompt GEMM kernels, RMSNorm), qtts_int8.hip (8-bit rows, weights and products), qtts_attention.hip, qtts_glue.hip
+(picks, gathers, per-frame glue) and qtts_model.hip (the decoder stack, graphs).  They are compiled side by side and linked into one shared object.
 
 --tuning builds tools/libqtts_hip_tuning.so instead (-DQTTS_TUNING: dispatch thresholds as settable globals, in-kernel
 timestamps, the grid-barrier probe, a stand-alone prompt-GEMM entry) for the measurement scripts under tools/, which
@@ -17,7 +17,7 @@ from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(os.path.dirname(HERE))
-UNITS = ["qtts_gemm.hip", "qtts_attention.hip", "qtts_glue.hip", "qtts_model.hip"]
+UNITS = ["qtts_gemm.hip", "qtts_int8.hip", "qtts_attention.hip", "qtts_glue.hip", "qtts_model.hip"]
 SRC = [os.path.join(HERE, u) for u in UNITS]
 OUT = os.path.join(HERE, "libqtts_hip.so")
 OUT_TUNING = os.path.join(ROOT, "tools", "libqtts_hip_tuning.so")

@@ -1,0 +1,398 @@
+// qtts_int8.hip - the 8-bit integer path: rows quantised with one scale each (alone, or behind the residual addition and
+// RMSNorm), int8 weight packing, and the product of int8 rows with int8 weights on the int8 matrix instructions, plain
+// or with the SwiGLU epilogue.  An extension: the reference has bf16 only.
+//
+//   s_m = max(max_k |y_mk| / 127, 2^-126)      q_mk = rint(y_mk / s_m)            |q| <= 127
+//   out_mn = bf16(xs_m * ws_n * sum_k q_mk w_nk [+ bias_n] [+ residual_mn])
+//
+// The sum is exact: |q w| <= 2^14, so int32 holds K <= 131071 of them whatever the order of the additions - the same
+// result for every tile shape and every split of K, which is why the launch is free to choose both by speed alone.
+// Everything after the sum is fp32 with one rounding to bf16 at the store.
+#include "qtts_common.h"
+
+typedef int int4_t __attribute__((ext_vector_type(4)));
+
+static constexpr int I8_MAX_K = 131071;            // int32 holds the sum of this many products of two int8 values
+static constexpr float I8_TINY = 0x1p-126f;        // smallest scale: its reciprocal is finite, rows of zeros stay zeros
+
+__host__ __device__ static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+// ------------------------------------------------------------------ rows -> int8
+struct RowsI8Args {
+    const bf16_t *x; int ldx;
+    const bf16_t *delta; int ldd;
+    const bf16_t *w; float eps;
+    bf16_t *sum; int lds;
+    int8_t *q; int ldq;
+    float *scales;
+    int M, K;
+};
+
+// 8 columns from k0 on of a row; columns behind the last are zeros.  VEC: rows are 16-byte aligned.
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const bf16_t *row, int k0, int K) {
+    if (VEC && k0 + 8 <= K) return *reinterpret_cast<const uint4 *>(row + k0);
+    Frag f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f.h[j] = k0 + j < K ? row[k0 + j] : (bf16_t)0;
+    return f.u;
+}
+template <bool VEC>
+__device__ __forceinline__ void store8(bf16_t *row, int k0, int K, uint4 v) {
+    if (VEC && k0 + 8 <= K) { *reinterpret_cast<uint4 *>(row + k0) = v; return; }
+    Frag f;
+    f.u = v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) if (k0 + j < K) row[k0 + j] = f.h[j];
+}
+
+// Four values of at most 127.5 in magnitude, rounded to the nearest integer (ties to even) and packed: 1.5 * 2^23 + v has
+// the integer in its low bits, in two's complement.
+__device__ __forceinline__ uint32_t pack4_i8(float a, float b, float c, float d) {
+    const float magic = 12582912.0f;
+    const uint32_t ua = __float_as_uint(a + magic), ub = __float_as_uint(b + magic);
+    const uint32_t uc = __float_as_uint(c + magic), ud = __float_as_uint(d + magic);
+    const uint32_t lo = __builtin_amdgcn_perm(ub, ua, 0x0c0c0400), hi = __builtin_amdgcn_perm(ud, uc, 0x0c0c0400);
+    return lo | (hi << 16);
+}
+
+// A row per T = 64 * W threads; thread t holds the 8-column chunks t, t + T, ... (CH of them) as bf16 across both
+// reductions, so x, delta and the weights are read once and nothing is read back.
+template <int W, int CH, bool NORM, bool VEC>
+__global__ __launch_bounds__(W * 64) void rows_int8_kernel(RowsI8Args a) {
+    constexpr int T = W * 64;
+    __shared__ float red_f[W];
+    __shared__ uint32_t red_u[W];
+    const int t = threadIdx.x;
+    for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
+        const bf16_t *xr = a.x + (size_t)m * a.ldx;
+        Frag h[CH], wv[CH];
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int k0 = (c * T + t) * 8;
+            h[c].u = k0 < a.K ? load8<VEC>(xr, k0, a.K) : make_uint4(0, 0, 0, 0);
+        }
+        if (NORM && a.delta) {
+            const bf16_t *dr = a.delta + (size_t)m * a.ldd;
+            bf16_t *sr = a.sum + (size_t)m * a.lds;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int k0 = (c * T + t) * 8;
+                if (k0 >= a.K) continue;
+                Frag d;
+                d.u = load8<VEC>(dr, k0, a.K);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) h[c].h[j] = f2bf(bf2f(h[c].h[j]) + bf2f(d.h[j]));
+                store8<VEC>(sr, k0, a.K, h[c].u);
+            }
+        }
+        float rstd = 1.0f;
+        if (NORM) {
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+                const int k0 = (c * T + t) * 8;
+                wv[c].u = k0 < a.K ? load8<VEC>(a.w, k0, a.K) : make_uint4(0, 0, 0, 0);
+            }
+            float ss = 0.f;
+#pragma unroll
+            for (int c = 0; c < CH; ++c) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { const float v = bf2f(h[c].h[j]); ss += v * v; }
+            }
+            for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+            if (W > 1) {
+                if ((t & 63) == 0) red_f[t >> 6] = ss;
+                __syncthreads();
+                ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < W; ++i) ss += red_f[i];
+            }
+            rstd = 1.0f / sqrtf(ss / (float)a.K + a.eps);
+        }
+        // the largest magnitude as an integer maximum over the numbers' bits: a NaN is above every number and stays
+        uint32_t top = 0;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                float v = bf2f(h[c].h[j]);
+                if (NORM) v = v * rstd * bf2f(wv[c].h[j]);
+                // columns behind the last are zeros, also where rstd is not finite
+                if (NORM && !((c * T + t) * 8 + j < a.K)) v = 0.f;
+                top = max(top, __float_as_uint(v) & 0x7fffffffu);
+            }
+        }
+        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+        if (W > 1) {
+            if ((t & 63) == 0) red_u[t >> 6] = top;
+            __syncthreads();
+            top = 0;
+#pragma unroll
+            for (int i = 0; i < W; ++i) top = max(top, red_u[i]);
+            if (m + gridDim.x < (unsigned)a.M) __syncthreads();      // the next row writes red_* again
+        }
+        float s = __uint_as_float(top) / 127.0f;
+        if (s < I8_TINY) s = I8_TINY;                     // NaN and infinity stay: the whole row then stands for NaN
+        const float inv = top < 0x7f800000u ? 1.0f / s : 0.f;
+        if (t == 0) a.scales[m] = s;
+        int8_t *qr = a.q + (size_t)m * a.ldq;
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int k0 = (c * T + t) * 8;
+            if (k0 >= a.K) continue;
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = bf2f(h[c].h[j]);
+                if (NORM) v[j] = v[j] * rstd * bf2f(wv[c].h[j]);
+                v[j] = inv != 0.f ? v[j] * inv : 0.f;     // a row that is not finite: zeros
+            }
+            const uint2 p = make_uint2(pack4_i8(v[0], v[1], v[2], v[3]), pack4_i8(v[4], v[5], v[6], v[7]));
+            if (k0 + 8 <= a.K) *reinterpret_cast<uint2 *>(qr + k0) = p;
+            else
+                for (int j = 0; j < a.K - k0; ++j) qr[k0 + j] = (int8_t)((j < 4 ? p.x >> (8 * j) : p.y >> (8 * (j - 4))) & 0xff);
+        }
+    }
+}
+
+template <bool NORM, bool VEC>
+static void launch_rows_int8(const RowsI8Args &a, hipStream_t s) {
+    const dim3 grid(std::min(a.M, 1 << 20));       // rows beyond that in turns: a launch takes fewer than 2^32 threads
+#define QTTS_ROWS_I8(W, CH) if (a.K <= W * 64 * 8 * CH) { \
+        hipLaunchKernelGGL((rows_int8_kernel<W, CH, NORM, VEC>), grid, dim3(W * 64), 0, s, a); return; }
+    QTTS_ROWS_I8(4, 1)
+    QTTS_ROWS_I8(4, 2)
+    QTTS_ROWS_I8(4, 4)
+    QTTS_ROWS_I8(16, 2)
+    QTTS_ROWS_I8(16, 4)
+    QTTS_ROWS_I8(16, 8)
+    QTTS_ROWS_I8(16, 16)
+#undef QTTS_ROWS_I8
+}
+
+extern "C" int qtts_quantize_int8(const void *x, int ldx, void *q, int ldq, float *scales, int M, int K, qtts_stream_t stream) {
+    QCHECK(x && q && scales, "quantize_int8: null pointer");
+    QCHECK(M > 0 && K > 0 && K <= I8_MAX_K, "quantize_int8: bad shape M=%d K=%d (K <= %d)", M, K, I8_MAX_K);
+    QCHECK(ldx >= K && ldq >= K && ldq % 16 == 0, "quantize_int8: row strides ldx=%d ldq=%d (need ldx >= K, ldq >= K, ldq %% 16 == 0)", ldx, ldq);
+    QCHECK(((uintptr_t)x & 1) == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)scales & 3) == 0, "quantize_int8: misaligned pointer");
+    RowsI8Args a{};
+    a.x = (const bf16_t *)x; a.ldx = ldx; a.q = (int8_t *)q; a.ldq = ldq; a.scales = scales; a.M = M; a.K = K;
+    if (((uintptr_t)x & 15) == 0 && ldx % 8 == 0) launch_rows_int8<false, true>(a, (hipStream_t)stream);
+    else launch_rows_int8<false, false>(a, (hipStream_t)stream);
+    QLAUNCH();
+    return QTTS_OK;
+}
+
+extern "C" int qtts_rmsnorm_int8(const void *x, int ldx, const void *delta, int ldd, const void *w, float eps, void *sum, int lds,
+                                 void *q, int ldq, float *scales, int M, int H, qtts_stream_t stream) {
+    QCHECK(x && w && q && scales, "rmsnorm_int8: null pointer");
+    QCHECK(!delta == !sum, "rmsnorm_int8: delta and sum come together");
+    QCHECK(M > 0 && H > 0 && H <= I8_MAX_K, "rmsnorm_int8: bad shape M=%d H=%d (H <= %d)", M, H, I8_MAX_K);
+    QCHECK(ldx >= H && ldq >= H && ldq % 16 == 0 && (!delta || (ldd >= H && lds >= H)),
+           "rmsnorm_int8: row strides ldx=%d ldd=%d lds=%d ldq=%d (need >= H, ldq %% 16 == 0)", ldx, ldd, lds, ldq);
+    QCHECK((((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)sum) & 1) == 0 && ((uintptr_t)q & 15) == 0 &&
+           ((uintptr_t)scales & 3) == 0, "rmsnorm_int8: misaligned pointer");
+    RowsI8Args a{};
+    a.x = (const bf16_t *)x; a.ldx = ldx; a.delta = (const bf16_t *)delta; a.ldd = ldd; a.w = (const bf16_t *)w; a.eps = eps;
+    a.sum = (bf16_t *)sum; a.lds = lds; a.q = (int8_t *)q; a.ldq = ldq; a.scales = scales; a.M = M; a.K = H;
+    const bool vec = (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)sum) & 15) == 0 && ldx % 8 == 0 &&
+                     (!delta || (ldd % 8 == 0 && lds % 8 == 0));
+    if (vec) launch_rows_int8<true, true>(a, (hipStream_t)stream);
+    else launch_rows_int8<true, false>(a, (hipStream_t)stream);
+    QLAUNCH();
+    return QTTS_OK;
+}
+
+// ------------------------------------------------------------------ weight packing
+// packed[tile][k-step][lane][16 B]: lane (g, r) of k-step ks holds row 16 * tile + r, columns 64 * ks + 16 * g .. +16 - the
+// 16 bytes a lane feeds to v_mfma_i32_16x16x64_i8.  Rows and columns behind the last are zeros; k-steps come in pairs.
+// gate/up: the tile's packed row 4 * p + j holds output i = 8 * tile + 2 * p + (j & 1), gate for j < 2 and up for j >= 2: a
+// lane's four sums are two gates and the two ups of the same outputs, and the epilogue needs no other lane.
+static inline int i8_ksteps(int K) { return 2 * ceil_div(K, 128); }
+
+__global__ __launch_bounds__(256) void pack_int8_kernel(const int8_t *__restrict__ w, const int8_t *__restrict__ up, int ldw,
+                                                        uint4 *__restrict__ packed, int N, int K, int ksteps, size_t total) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (size_t)gridDim.x * 256) {
+        const int lane = i & 63;
+        const size_t rest = i >> 6;
+        const int ks = (int)(rest % ksteps), tile = (int)(rest / ksteps), r = lane & 15, k0 = 64 * ks + 16 * (lane >> 4);
+        const int n = up ? 8 * tile + 2 * (r >> 2) + (r & 1) : 16 * tile + r;
+        const int8_t *src = (up && (r & 2) ? up : w) + (size_t)n * ldw;
+        union { uint4 u; int8_t b[16]; } v;
+        v.u = make_uint4(0, 0, 0, 0);
+        if (n < N)
+            for (int j = 0; j < 16; ++j) if (k0 + j < K) v.b[j] = src[k0 + j];
+        packed[i] = v.u;
+    }
+}
+
+extern "C" size_t qtts_packed_weight_int8_bytes(int N, int K) {
+    if (N <= 0 || K <= 0 || N > 0x7ffffff0 || K > I8_MAX_K) return 0;
+    return (size_t)ceil_div(N, 16) * i8_ksteps(K) * 1024;
+}
+extern "C" size_t qtts_packed_gate_up_int8_bytes(int I, int K) {
+    if (I <= 0 || K <= 0 || I > 0x3ffffff0 || K > I8_MAX_K) return 0;
+    return (size_t)ceil_div(I, 8) * i8_ksteps(K) * 1024;
+}
+
+static int pack_int8(const char *who, const void *w, const void *up, int ldw, void *packed, int N, int K, int tiles, hipStream_t s) {
+    QCHECK(N > 0 && K > 0 && K <= I8_MAX_K && ldw >= K, "%s: bad shape N=%d K=%d ldw=%d (K <= %d)", who, N, K, ldw, I8_MAX_K);
+    QCHECK(((uintptr_t)packed & 15) == 0, "%s: misaligned pointer", who);
+    const size_t total = (size_t)tiles * i8_ksteps(K) * 64;
+    hipLaunchKernelGGL(pack_int8_kernel, dim3((unsigned)std::min<size_t>((total + 255) / 256, 1 << 20)), dim3(256), 0, s,
+                       (const int8_t *)w, (const int8_t *)up, ldw, (uint4 *)packed, N, K, i8_ksteps(K), total);
+    QLAUNCH();
+    return QTTS_OK;
+}
+extern "C" int qtts_pack_weight_int8(const void *w, int ldw, void *packed, int N, int K, qtts_stream_t stream) {
+    QCHECK(w && packed, "pack_weight_int8: null pointer");
+    return pack_int8("pack_weight_int8", w, nullptr, ldw, packed, N, K, ceil_div(N, 16), (hipStream_t)stream);
+}
+extern "C" int qtts_pack_gate_up_int8(const void *gate, const void *up, int ldw, void *packed, int I, int K, qtts_stream_t stream) {
+    QCHECK(gate && up && packed, "pack_gate_up_int8: null pointer");
+    return pack_int8("pack_gate_up_int8", gate, up, ldw, packed, I, K, ceil_div(I, 8), (hipStream_t)stream);
+}
+
+// ------------------------------------------------------------------ the product
+struct LinI8Args {
+    const int8_t *x; int ldx;
+    const float *xs;
+    const uint4 *wp;
+    const float *ws, *us;          // scales per output channel; SwiGLU: of the gate and the up rows
+    const bf16_t *bias, *res; int ldr;
+    bf16_t *out; int ldo;
+    int M, N, K, ksteps;           // N: output columns; ksteps: of a packed tile
+    int ov, rv;                    // 8-byte (SwiGLU: 4-byte) stores / residual loads are aligned
+};
+
+// One 16 x 16 tile of sums, this lane's four of them: weight rows 4 * (lane / 16) .. +3 of `tile`, activation row m.
+template <bool SWIGLU>
+__device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int tile, int m, int lane) {
+    if (m >= a.M) return;
+    const float xs = a.xs[m];
+    bf16_t *o = a.out + (size_t)m * a.ldo;
+    if (SWIGLU) {
+        const int n = 8 * tile + 2 * (lane >> 4);
+        float y[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int nn = min(n + j, a.N - 1);
+            y[j] = silu_f((float)acc[j] * xs * a.ws[nn]) * ((float)acc[2 + j] * xs * a.us[nn]);
+        }
+        if (a.ov && n + 2 <= a.N) *reinterpret_cast<uint32_t *>(o + n) = pack2(y[0], y[1]);
+        else
+            for (int j = 0; j < 2; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
+        return;
+    }
+    const int n = 16 * tile + 4 * (lane >> 4);
+    float y[4];
+    const bool full = n + 4 <= a.N;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int nn = min(n + j, a.N - 1);
+        y[j] = (float)acc[j] * xs * a.ws[nn];
+        if (a.bias) y[j] += bf2f(a.bias[nn]);
+    }
+    if (a.res) {
+        const bf16_t *rr = a.res + (size_t)m * a.ldr;
+        if (a.rv && full) {
+            const uint2 r = *reinterpret_cast<const uint2 *>(rr + n);
+            float p, q;
+            unpack2(r.x, p, q); y[0] += p; y[1] += q;
+            unpack2(r.y, p, q); y[2] += p; y[3] += q;
+        } else
+            for (int j = 0; j < 4; ++j) y[j] += bf2f(rr[min(n + j, a.N - 1)]);
+    }
+    if (a.ov && full) *reinterpret_cast<uint2 *>(o + n) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+    else
+        for (int j = 0; j < 4; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
+}
+
+union I8Frag { uint4 u; int4_t v; };
+
+// Few rows: a workgroup owns TM row tiles x TN weight tiles and its NW waves share K, each wave a contiguous run of
+// k-steps straight from memory to registers; the waves' sums meet in LDS.
+template <int TM, int TN, int NW, bool SWIGLU>
+__global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a) {
+    __shared__ int4_t red[NW][TM * TN][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int tiles = SWIGLU ? ceil_div(a.N, 8) : ceil_div(a.N, 16);
+    const int t0 = blockIdx.x * TN, m0 = blockIdx.y * TM * 16;
+    const int steps = ceil_div(a.K, 64), per = ceil_div(steps, NW), ks0 = wave * per, ks1 = min(steps, ks0 + per);
+    const int8_t *xp[TM];
+    const uint4 *wp[TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i) xp[i] = a.x + (size_t)min(m0 + 16 * i + r, a.M - 1) * a.ldx;
+#pragma unroll
+    for (int i = 0; i < TN; ++i) wp[i] = a.wp + (size_t)min(t0 + i, tiles - 1) * a.ksteps * 64 + lane;
+    int4_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = int4_t{0, 0, 0, 0};
+    for (int ks = ks0; ks < ks1; ++ks) {
+        I8Frag xf[TM], wf[TN];
+        const int k = 64 * ks + 16 * g, kk = k < a.K ? k : 0;      // behind the last column the packed weights are zeros
+#pragma unroll
+        for (int i = 0; i < TM; ++i) xf[i].u = *reinterpret_cast<const uint4 *>(xp[i] + kk);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) wf[i].u = wp[i][(size_t)ks * 64];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) red[wave][i * TN + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int t = wave; t < TM * TN; t += NW) {
+        int4_t sum = red[0][t][lane];
+#pragma unroll
+        for (int w = 1; w < NW; ++w) sum += red[w][t][lane];
+        if (t0 + t % TN < tiles) i8_store<SWIGLU>(a, sum, t0 + t % TN, m0 + 16 * (t / TN) + r, lane);
+    }
+}
+
+static int launch_linear_int8(const char *who, LinI8Args a, bool swiglu, hipStream_t s) {
+    const int tiles = ceil_div(a.N, swiglu ? 8 : 16), rt = ceil_div(a.M, 16);
+    QCHECK(ceil_div(rt, 4) <= 65535, "%s: M=%d", who, a.M);
+    if (swiglu) hipLaunchKernelGGL((linear_int8_split_kernel<4, 2, 8, true>), dim3(ceil_div(tiles, 2), ceil_div(rt, 4)), dim3(512), 0, s, a);
+    else hipLaunchKernelGGL((linear_int8_split_kernel<4, 2, 8, false>), dim3(ceil_div(tiles, 2), ceil_div(rt, 4)), dim3(512), 0, s, a);
+    QLAUNCH();
+    return QTTS_OK;
+}
+
+static int linear_int8_checked(const char *who, const void *x, int ldx, const float *xs, const void *wp, const float *ws,
+                               const float *us, const void *bias, const void *res, int ldr, void *out, int ldo, int M, int N,
+                               int K, bool swiglu, qtts_stream_t stream) {
+    QCHECK(x && xs && wp && ws && out && (!swiglu || us), "%s: null pointer", who);
+    QCHECK(M > 0 && N > 0 && K > 0 && K <= I8_MAX_K && N <= 0x3ffffff0, "%s: bad shape M=%d N=%d K=%d (K <= %d)", who, M, N, K, I8_MAX_K);
+    QCHECK(ldx % 16 == 0 && ldx >= K, "%s: x row stride %d too small or not a multiple of 16", who, ldx);
+    QCHECK(ldo >= N && (!res || ldr >= N), "%s: row strides ldo=%d ldr=%d < N=%d", who, ldo, ldr, N);
+    QCHECK((((uintptr_t)x | (uintptr_t)wp) & 15) == 0 && (((uintptr_t)xs | (uintptr_t)ws | (uintptr_t)us) & 3) == 0 &&
+           (((uintptr_t)out | (uintptr_t)bias | (uintptr_t)res) & 1) == 0, "%s: misaligned pointer", who);
+    LinI8Args a{};
+    a.x = (const int8_t *)x; a.ldx = ldx; a.xs = xs; a.wp = (const uint4 *)wp; a.ws = ws; a.us = us;
+    a.bias = (const bf16_t *)bias; a.res = (const bf16_t *)res; a.ldr = ldr; a.out = (bf16_t *)out; a.ldo = ldo;
+    a.M = M; a.N = N; a.K = K; a.ksteps = i8_ksteps(K);
+    const int pitch = swiglu ? 2 : 4;
+    a.ov = ((uintptr_t)out & (2 * pitch - 1)) == 0 && ldo % pitch == 0;
+    a.rv = ((uintptr_t)res & 7) == 0 && ldr % 4 == 0;
+    return launch_linear_int8(who, a, swiglu, (hipStream_t)stream);
+}
+
+extern "C" int qtts_linear_int8(const void *x, int ldx, const float *x_scales, const void *w_packed, const float *w_scales,
+                                const void *bias, const void *residual, int ldr, void *out, int ldo, int M, int N, int K,
+                                qtts_stream_t stream) {
+    return linear_int8_checked("linear_int8", x, ldx, x_scales, w_packed, w_scales, nullptr, bias, residual, ldr, out, ldo, M, N, K,
+                               false, stream);
+}
+
+extern "C" int qtts_linear_swiglu_int8(const void *x, int ldx, const float *x_scales, const void *w_gate_up_packed,
+                                       const float *gate_scales, const float *up_scales, void *out, int ldo, int M, int I, int K,
+                                       qtts_stream_t stream) {
+    return linear_int8_checked("linear_swiglu_int8", x, ldx, x_scales, w_gate_up_packed, gate_scales, up_scales, nullptr, nullptr, 0,
+                               out, ldo, M, I, K, true, stream);
+}
