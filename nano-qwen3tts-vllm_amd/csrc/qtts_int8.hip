@@ -262,8 +262,14 @@ struct LinI8Args {
     const bf16_t *bias, *res; int ldr;
     bf16_t *out; int ldo;
     int M, N, K, ksteps;           // N: output columns; ksteps: of a packed tile
-    int ov, rv;                    // 8-byte (SwiGLU: 4-byte) stores / residual loads are aligned
+    int ov, rv;                    // output / residual rows: bytes they are aligned to
 };
+
+// What follows a sum, in the same operations in every kernel: a row's result does not depend on the form it came from.
+__device__ __forceinline__ float i8_scaled(int acc, float xs, float ws, float bias) { return __builtin_fmaf((float)acc * xs, ws, bias); }
+__device__ __forceinline__ float i8_swiglu(int g, int u, float xs, float gs, float us) {
+    return silu_f((float)g * xs * gs) * ((float)u * xs * us);
+}
 
 // One 16 x 16 tile of sums, this lane's four of them: weight rows 4 * (lane / 16) .. +3 of `tile`, activation row m.
 template <bool SWIGLU>
@@ -277,9 +283,9 @@ __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int til
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int nn = min(n + j, a.N - 1);
-            y[j] = silu_f((float)acc[j] * xs * a.ws[nn]) * ((float)acc[2 + j] * xs * a.us[nn]);
+            y[j] = i8_swiglu(acc[j], acc[2 + j], xs, a.ws[nn], a.us[nn]);
         }
-        if (a.ov && n + 2 <= a.N) *reinterpret_cast<uint32_t *>(o + n) = pack2(y[0], y[1]);
+        if (a.ov >= 4 && n + 2 <= a.N) *reinterpret_cast<uint32_t *>(o + n) = pack2(y[0], y[1]);
         else
             for (int j = 0; j < 2; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
         return;
@@ -290,12 +296,11 @@ __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int til
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int nn = min(n + j, a.N - 1);
-        y[j] = (float)acc[j] * xs * a.ws[nn];
-        if (a.bias) y[j] += bf2f(a.bias[nn]);
+        y[j] = i8_scaled(acc[j], xs, a.ws[nn], a.bias ? bf2f(a.bias[nn]) : 0.f);
     }
     if (a.res) {
         const bf16_t *rr = a.res + (size_t)m * a.ldr;
-        if (a.rv && full) {
+        if (a.rv >= 8 && full) {
             const uint2 r = *reinterpret_cast<const uint2 *>(rr + n);
             float p, q;
             unpack2(r.x, p, q); y[0] += p; y[1] += q;
@@ -303,7 +308,7 @@ __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int til
         } else
             for (int j = 0; j < 4; ++j) y[j] += bf2f(rr[min(n + j, a.N - 1)]);
     }
-    if (a.ov && full) *reinterpret_cast<uint2 *>(o + n) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+    if (a.ov >= 8 && full) *reinterpret_cast<uint2 *>(o + n) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
     else
         for (int j = 0; j < 4; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
 }
@@ -355,13 +360,229 @@ __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a)
     }
 }
 
+#pragma clang diagnostic ignored "-Winline-asm"     // "reserved register" m0 in a clobber list: it is what the block writes
+// 16 bytes per lane from memory to LDS, lane i's to place i behind the LDS address `at` (the same in every lane).  In
+// assembly because the compiler, which sees a write to LDS in the builtin, waits for it in front of the next read of any
+// LDS; here the waits are the caller's: s_waitcnt vmcnt before the barrier in front of the reads.  M0 written by the scalar
+// unit is seen by the request one wait state later.
+__device__ __forceinline__ void lds_request16(const void *from, uint32_t at) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
+}
+__device__ __forceinline__ uint32_t lds_address(const void *p) {
+    return __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void *)p);
+}
+
+// Many rows: a workgroup owns BM activation rows x BN weight rows (packed order) and its WM x WN waves an equal part each.
+// KS k-steps (64 columns each) of both go to LDS at a time, straight from memory, 16 bytes a lane; ST stages of LDS, so ST - 1
+// of them are on their way while one is multiplied.  The weights keep their fragment order; the rows of a 1 KiB request (16
+// rows x 64 columns or 8 x 128) stay row-major, the 16-byte chunk c of row r at place c ^ swizzle(r), so that the 16 rows a
+// fragment read touches lie in 16 different places modulo 256 bytes.
+template <int KS>
+__device__ __forceinline__ int i8_swizzle(int r) { return KS == 1 ? (r >> 2) & 3 : (r >> 1) & 7; }
+
+template <int N>
+__device__ __forceinline__ void wait_and_meet() {
+    // this wave's requests but the last N are in and its reads of LDS are done; behind the barrier, everybody's
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
+
+template <int BM, int BN, int WM, int WN, int KS, int ST, bool SWIGLU>
+__global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Args a, int mtiles, int ntiles) {
+    constexpr int NW = WM * WN, RPR = 16 / KS, CPR = 4 * KS;       // rows of a request, 16-byte chunks of a row
+    constexpr int NA = BM / RPR / NW, NB = BN / 16 * KS / NW, TM = BM / WM / 16, TN = BN / WN / 16;
+    constexpr int STAGE = (BM + BN) * CPR;                         // 16-byte places of a stage
+    static_assert(BM % (RPR * NW) == 0 && (BN / 16 * KS) % NW == 0 && (RPR * NW) % 16 == 0, "whole requests per wave");
+    static_assert((ST - 2) * (NA + NB) <= 63, "the wait counter's range");
+    __shared__ uint4 lds[ST * STAGE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int id = blockIdx.x;
+    const int total = mtiles * ntiles;
+    if (total % 8 == 0) id = (id & 7) * (total >> 3) + (id >> 3);      // workgroups are dealt to the 8 XCDs in turn
+    const int mt = id / ntiles, nt = id % ntiles;
+    const int m0 = mt * BM, t0 = nt * (BN / 16);
+    const int tiles = SWIGLU ? ceil_div(a.N, 8) : ceil_div(a.N, 16);
+    const int8_t *xp[NA];
+    const int rr = lane / CPR, chunk = (lane % CPR) ^ i8_swizzle<KS>(RPR * wave + rr);
+#pragma unroll
+    for (int i = 0; i < NA; ++i) xp[i] = a.x + (size_t)min(m0 + RPR * (wave + i * NW) + rr, a.M - 1) * a.ldx;
+    const uint4 *wp[NB];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+        const int v = wave + i * NW;
+        wp[i] = a.wp + ((size_t)min(t0 + v / KS, tiles - 1) * a.ksteps + v % KS) * 64 + lane;
+    }
+    const uint32_t lds_at = lds_address(lds) + wave * 1024;
+    auto request = [&](int it, int stage) {
+        const int k = 64 * KS * it + 16 * chunk, kk = k < a.K ? k : 0;
+        const uint32_t to = lds_at + stage * (STAGE * 16);
+#pragma unroll
+        for (int i = 0; i < NA; ++i) lds_request16(xp[i] + kk, to + i * NW * 1024);
+#pragma unroll
+        for (int i = 0; i < NB; ++i) lds_request16(wp[i] + (size_t)it * (64 * KS), to + BM * CPR * 16 + i * NW * 1024);
+    };
+    const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
+    const int xat = (wm * TM * 16 + r) * CPR + (g ^ i8_swizzle<KS>(r)), wat = BM * CPR + wn * TN * 64 * KS + lane;
+    int4_t acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = int4_t{0, 0, 0, 0};
+    const int nk = a.ksteps / KS;
+#pragma unroll
+    for (int i = 0; i < ST - 1; ++i) if (i < nk) request(i, i);
+    int stage = 0, next = ST - 1;
+    for (int it = 0; it < nk; ++it) {
+        if (it + ST - 2 < nk) wait_and_meet<(ST - 2) * (NA + NB)>();
+        else wait_and_meet<0>();
+        if (it + ST - 1 < nk) request(it + ST - 1, next);
+        const uint4 *st = lds + stage * STAGE;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            I8Frag xf[TM], wf[TN];
+#pragma unroll
+            for (int j = 0; j < TN; ++j) wf[j].u = st[wat + j * 64 * KS + s * 64];
+#pragma unroll
+            for (int i = 0; i < TM; ++i) xf[i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
+        }
+        stage = stage + 1 == ST ? 0 : stage + 1;
+        next = next + 1 == ST ? 0 : next + 1;
+    }
+    // Epilogue.  A wave turns its sums round in LDS of its own, HT row tiles at a time, so that a lane has eight neighbouring
+    // outputs of a row: 16-byte loads and stores, and the same columns - hence the same scales and bias, in registers - in
+    // every pass.  The loop over the passes is kept rolled: unrolled over the tile's sums it was 48 KB of code, fetched once per
+    // workgroup, and took 13 us of a 49 us launch.
+    asm volatile("s_barrier" ::: "memory");
+    constexpr int CP = SWIGLU ? 16 : 8, LPR = TN * 16 / CP, PITCH = TN * 16 + 4, RPP = 64 / LPR;
+    constexpr int HT0 = ST * STAGE * 4 / (NW * 16 * PITCH), HT = HT0 >= TM ? TM : HT0 >= 4 && TM % 4 == 0 ? 4 : HT0 >= 2 && TM % 2 == 0 ? 2 : 1;
+    static_assert(HT0 >= 1 && TM % HT == 0 && (16 * HT) % RPP == 0, "whole passes");
+    int *mine = reinterpret_cast<int *>(lds) + wave * HT * 16 * PITCH;
+    const int c = lane % LPR, n0 = (t0 + wn * TN) * (SWIGLU ? 8 : 16) + 8 * c;       // this lane's outputs n0 .. n0 + 7
+    float s0[8], s1[8];                                                              // scales; SwiGLU: up scales, else bias
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const int n = min(n0 + j, a.N - 1);
+        s0[j] = a.ws[n];
+        s1[j] = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
+    }
+    const bool whole = n0 + 8 <= a.N, wide = whole && a.ov == 16, rwide = whole && a.rv == 16;
+#pragma unroll
+    for (int h = 0; h < TM; h += HT) {
+#pragma unroll
+        for (int i = 0; i < HT; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) *reinterpret_cast<int4_t *>(mine + (16 * i + r) * PITCH + 16 * j + 4 * g) = acc[h + i][j];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int p = 0; p < 16 * HT / RPP; ++p) {
+            const int row = p * RPP + lane / LPR, m = m0 + (wm * TM + h) * 16 + row;
+            const int4_t *v = reinterpret_cast<const int4_t *>(mine + row * PITCH + CP * c);
+            if (m >= a.M || n0 >= a.N) continue;
+            const float xs = a.xs[m];
+            float y[8];
+            if (SWIGLU) {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int4_t t = v[q];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) y[2 * q + j] = i8_swiglu(t[j], t[2 + j], xs, s0[2 * q + j], s1[2 * q + j]);
+                }
+            } else {
+                const int4_t lo = v[0], hi = v[1];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    y[j] = i8_scaled(lo[j], xs, s0[j], s1[j]);
+                    y[4 + j] = i8_scaled(hi[j], xs, s0[4 + j], s1[4 + j]);
+                }
+                if (a.res) {
+                    const bf16_t *rr = a.res + (size_t)m * a.ldr + n0;
+                    Frag f;
+                    if (rwide) f.u = *reinterpret_cast<const uint4 *>(rr);
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) f.h[j] = n0 + j < a.N ? rr[j] : (bf16_t)0;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) y[j] += bf2f(f.h[j]);
+                }
+            }
+            Frag f;
+            f.u = make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
+            bf16_t *o = a.out + (size_t)m * a.ldo + n0;
+            if (wide) *reinterpret_cast<uint4 *>(o) = f.u;
+            else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) if (n0 + j < a.N) o[j] = f.h[j];
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// The forms a product may take, by number (a measurement build may force one: qtts_tune_int8)
+#ifdef QTTS_TUNING
+static int g_i8_form = 0;
+extern "C" void qtts_tune_int8(int form) { g_i8_form = form; }
+#else
+static constexpr int g_i8_form = 0;
+#endif
+
+template <bool SWIGLU>
+static void launch_form_int8(const LinI8Args &a, int tiles, int form, hipStream_t s) {
+#define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \
+        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, SWIGLU>), dim3(mt * nt), dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
+#define QTTS_SPLIT_I8(TM, TN, NW) hipLaunchKernelGGL((linear_int8_split_kernel<TM, TN, NW, SWIGLU>), \
+        dim3(ceil_div(tiles, TN), ceil_div(a.M, 16 * TM)), dim3(NW * 64), 0, s, a)
+    switch (form) {
+    case 1: QTTS_SPLIT_I8(1, 1, 4); break;
+    case 2: QTTS_SPLIT_I8(1, 1, 8); break;
+    case 3: QTTS_SPLIT_I8(1, 2, 8); break;
+    case 4: QTTS_SPLIT_I8(2, 1, 8); break;
+    case 5: QTTS_SPLIT_I8(2, 2, 8); break;
+    case 6: QTTS_SPLIT_I8(4, 1, 8); break;
+    case 7: QTTS_SPLIT_I8(4, 2, 8); break;
+    case 8: QTTS_SPLIT_I8(2, 2, 4); break;
+    case 9: QTTS_SPLIT_I8(4, 2, 4); break;
+    case 10: QTTS_SPLIT_I8(2, 4, 8); break;
+    case 11: QTTS_SPLIT_I8(4, 4, 8); break;
+    case 12: QTTS_SPLIT_I8(4, 4, 4); break;
+    case 20: QTTS_TILE_I8(64, 64, 2, 2, 1, 4); break;
+    case 21: QTTS_TILE_I8(64, 64, 2, 2, 2, 4); break;
+    case 22: QTTS_TILE_I8(64, 64, 2, 2, 2, 8); break;
+    case 23: QTTS_TILE_I8(128, 128, 2, 2, 1, 5); break;
+    case 24: QTTS_TILE_I8(128, 128, 2, 2, 2, 4); break;
+    case 25: QTTS_TILE_I8(128, 128, 2, 2, 2, 5); break;
+    case 26: QTTS_TILE_I8(256, 256, 2, 4, 1, 3); break;
+    case 27: QTTS_TILE_I8(256, 256, 2, 4, 1, 4); break;
+    case 28: QTTS_TILE_I8(256, 256, 2, 4, 1, 5); break;
+    case 29: QTTS_TILE_I8(256, 256, 4, 2, 1, 4); break;
+    case 30: QTTS_TILE_I8(256, 256, 2, 4, 2, 2); break;
+    case 31: QTTS_TILE_I8(256, 128, 4, 2, 1, 6); break;
+    case 32: QTTS_TILE_I8(128, 256, 2, 4, 1, 3); break;
+    case 33: QTTS_TILE_I8(128, 128, 2, 4, 1, 4); break;
+    case 34: QTTS_TILE_I8(128, 64, 2, 2, 2, 4); break;
+    }
+#undef QTTS_TILE_I8
+#undef QTTS_SPLIT_I8
+}
+
 static int launch_linear_int8(const char *who, LinI8Args a, bool swiglu, hipStream_t s) {
-    const int tiles = ceil_div(a.N, swiglu ? 8 : 16), rt = ceil_div(a.M, 16);
-    QCHECK(ceil_div(rt, 4) <= 65535, "%s: M=%d", who, a.M);
-    if (swiglu) hipLaunchKernelGGL((linear_int8_split_kernel<4, 2, 8, true>), dim3(ceil_div(tiles, 2), ceil_div(rt, 4)), dim3(512), 0, s, a);
-    else hipLaunchKernelGGL((linear_int8_split_kernel<4, 2, 8, false>), dim3(ceil_div(tiles, 2), ceil_div(rt, 4)), dim3(512), 0, s, a);
+    const int tiles = ceil_div(a.N, swiglu ? 8 : 16);
+    const int form = g_i8_form ? g_i8_form : a.M >= 2048 ? 27 : a.M >= 512 ? 24 : 7;
+    QCHECK(form >= 20 || ceil_div(a.M, 16) <= 65535, "%s: M=%d", who, a.M);
+    if (swiglu) launch_form_int8<true>(a, tiles, form, s);
+    else launch_form_int8<false>(a, tiles, form, s);
     QLAUNCH();
     return QTTS_OK;
+}
+
+// The largest of 2, 4, 8, 16 that divides every row's address.
+static int row_alignment(const void *p, int ld) {
+    const uintptr_t bits = (uintptr_t)p | ((uintptr_t)ld * 2) | 16;
+    return (int)(bits & (~bits + 1));
 }
 
 static int linear_int8_checked(const char *who, const void *x, int ldx, const float *xs, const void *wp, const float *ws,
@@ -377,9 +598,8 @@ static int linear_int8_checked(const char *who, const void *x, int ldx, const fl
     a.x = (const int8_t *)x; a.ldx = ldx; a.xs = xs; a.wp = (const uint4 *)wp; a.ws = ws; a.us = us;
     a.bias = (const bf16_t *)bias; a.res = (const bf16_t *)res; a.ldr = ldr; a.out = (bf16_t *)out; a.ldo = ldo;
     a.M = M; a.N = N; a.K = K; a.ksteps = i8_ksteps(K);
-    const int pitch = swiglu ? 2 : 4;
-    a.ov = ((uintptr_t)out & (2 * pitch - 1)) == 0 && ldo % pitch == 0;
-    a.rv = ((uintptr_t)res & 7) == 0 && ldr % 4 == 0;
+    a.ov = row_alignment(out, ldo);
+    a.rv = row_alignment(res, ldr);
     return launch_linear_int8(who, a, swiglu, (hipStream_t)stream);
 }
 
