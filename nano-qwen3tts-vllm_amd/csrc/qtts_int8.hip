@@ -378,7 +378,12 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 // rows x 64 columns or 8 x 128) stay row-major, the 16-byte chunk c of row r at place c ^ swizzle(r), so that the 16 rows a
 // fragment read touches lie in 16 different places modulo 256 bytes.
 template <int KS>
-__device__ __forceinline__ int i8_swizzle(int r) { return KS == 1 ? (r >> 2) & 3 : (r >> 1) & 7; }
+__device__ __forceinline__ int i8_swizzle(int r) {
+    // A 16-byte read is served 16 lanes at a time: 0-3, 12-15, 20-23, 24-27, then 4-7, 8-11, 16-19, 28-31, and so on.  With
+    // 64-byte rows four rows share 256 bytes and the swizzle 0, 2, 3, 1 of the row quads keeps such a set apart (0, 1, 2, 3: two
+    // lanes to a place, and half the rate).
+    return KS == 1 ? ((r >> 1) & 2) ^ (((r >> 3) & 1) * 3) : (r >> 1) & 7;
+}
 
 template <int N>
 __device__ __forceinline__ void wait_and_meet() {
@@ -386,7 +391,7 @@ __device__ __forceinline__ void wait_and_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
-template <int BM, int BN, int WM, int WN, int KS, int ST, bool SWIGLU>
+template <int BM, int BN, int WM, int WN, int KS, int ST, bool ALT, bool SWIGLU>
 __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Args a, int mtiles, int ntiles) {
     constexpr int NW = WM * WN, RPR = 16 / KS, CPR = 4 * KS;       // rows of a request, 16-byte chunks of a row
     constexpr int NA = BM / RPR / NW, NB = BN / 16 * KS / NW, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -394,6 +399,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
     static_assert(BM % (RPR * NW) == 0 && (BN / 16 * KS) % NW == 0 && (RPR * NW) % 16 == 0, "whole requests per wave");
     static_assert((ST - 2) * (NA + NB) <= 63, "the wait counter's range");
     __shared__ uint4 lds[ST * STAGE];
+    __shared__ float xscale[BM];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int id = blockIdx.x;
     const int total = mtiles * ntiles;
@@ -401,6 +407,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
     const int mt = id / ntiles, nt = id % ntiles;
     const int m0 = mt * BM, t0 = nt * (BN / 16);
     const int tiles = SWIGLU ? ceil_div(a.N, 8) : ceil_div(a.N, 16);
+    for (int i = threadIdx.x; i < BM; i += NW * 64) xscale[i] = a.xs[min(m0 + i, a.M - 1)];
     const int8_t *xp[NA];
     const int rr = lane / CPR, chunk = (lane % CPR) ^ i8_swizzle<KS>(RPR * wave + rr);
 #pragma unroll
@@ -431,35 +438,84 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 #pragma unroll
     for (int i = 0; i < ST - 1; ++i) if (i < nk) request(i, i);
     int stage = 0, next = ST - 1;
-    for (int it = 0; it < nk; ++it) {
-        if (it + ST - 2 < nk) wait_and_meet<(ST - 2) * (NA + NB)>();
-        else wait_and_meet<0>();
-        if (it + ST - 1 < nk) request(it + ST - 1, next);
-        const uint4 *st = lds + stage * STAGE;
+    if (!ALT) {
+        for (int it = 0; it < nk; ++it) {
+            if (it + ST - 2 < nk) wait_and_meet<(ST - 2) * (NA + NB)>();
+            else wait_and_meet<0>();
+            if (it + ST - 1 < nk) request(it + ST - 1, next);
+            const uint4 *st = lds + stage * STAGE;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            I8Frag xf[TM], wf[TN];
+            for (int s = 0; s < KS; ++s) {
+                I8Frag xf[TM], wf[TN];
 #pragma unroll
-            for (int j = 0; j < TN; ++j) wf[j].u = st[wat + j * 64 * KS + s * 64];
+                for (int j = 0; j < TN; ++j) wf[j].u = st[wat + j * 64 * KS + s * 64];
 #pragma unroll
-            for (int i = 0; i < TM; ++i) xf[i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
+                for (int i = 0; i < TM; ++i) xf[i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
+            }
+            stage = stage + 1 == ST ? 0 : stage + 1;
+            next = next + 1 == ST ? 0 : next + 1;
         }
-        stage = stage + 1 == ST ? 0 : stage + 1;
-        next = next + 1 == ST ? 0 : next + 1;
+    } else {
+        // The two waves of a SIMD take turns: while one multiplies, the other reads its fragments of the next k-step, and a
+        // barrier after each turn keeps them so.  Turns: waves 0-3 read step k in turn 2k and multiply it in turn 2k + 1, waves
+        // 4-7 one turn later.  Stage k is complete before turn 2k: every wave waits for its own requests of it at the end of
+        // turn 2k - 1.  Requests into the place of stage k - 1, last read in turn 2k - 1, go out from turn 2k on.
+        const bool late = wave >= NW / 2;
+        if (ST - 1 <= nk) wait_and_meet<(ST - 2) * (NA + NB)>();
+        else wait_and_meet<0>();
+        if (late) asm volatile("s_barrier" ::: "memory");
+        for (int it = 0; it < nk; ++it) {
+            I8Frag xf[KS][TM], wf[KS][TN];
+            const uint4 *st = lds + stage * STAGE;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+#pragma unroll
+                for (int j = 0; j < TN; ++j) wf[s][j].u = st[wat + j * 64 * KS + s * 64];
+#pragma unroll
+                for (int i = 0; i < TM; ++i) xf[s][i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
+            }
+            const bool more = it + ST - 1 < nk;
+            if (more) request(it + ST - 1, next);
+            __builtin_amdgcn_sched_barrier(0);
+            if (late) {
+                if (more) wait_and_meet<(ST - 2) * (NA + NB)>();
+                else wait_and_meet<0>();
+            } else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[s][j].v, xf[s][i].v, acc[i][j], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (!late) {
+                if (more) wait_and_meet<(ST - 2) * (NA + NB)>();
+                else wait_and_meet<0>();
+            } else asm volatile("s_barrier" ::: "memory");
+            __builtin_amdgcn_sched_barrier(0);
+            stage = stage + 1 == ST ? 0 : stage + 1;
+            next = next + 1 == ST ? 0 : next + 1;
+        }
+        if (!late) asm volatile("s_barrier" ::: "memory");
     }
     // Epilogue.  A wave turns its sums round in LDS of its own, HT row tiles at a time, so that a lane has eight neighbouring
     // outputs of a row: 16-byte loads and stores, and the same columns - hence the same scales and bias, in registers - in
-    // every pass.  The loop over the passes is kept rolled: unrolled over the tile's sums it was 48 KB of code, fetched once per
-    // workgroup, and took 13 us of a 49 us launch.
-    asm volatile("s_barrier" ::: "memory");
-    constexpr int CP = SWIGLU ? 16 : 8, LPR = TN * 16 / CP, PITCH = TN * 16 + 4, RPP = 64 / LPR;
+    // every pass.  The passes stay a loop, PU of them at a time so that their residual rows are requested together: unrolled over
+    // the tile's sums the epilogue was 48 KB of code, fetched once per workgroup, and took 13 us of a 49 us launch.
+    // The 16-byte chunk c of row r lies at place c ^ r (modulo the chunks of a row, 16 at most).
+    constexpr int CP = SWIGLU ? 16 : 8, LPR = TN * 16 / CP, PITCH = TN * 16, RPP = 64 / LPR, CMASK = (TN * 4 < 16 ? TN * 4 : 16) - 1;
     constexpr int HT0 = ST * STAGE * 4 / (NW * 16 * PITCH), HT = HT0 >= TM ? TM : HT0 >= 4 && TM % 4 == 0 ? 4 : HT0 >= 2 && TM % 2 == 0 ? 2 : 1;
-    static_assert(HT0 >= 1 && TM % HT == 0 && (16 * HT) % RPP == 0, "whole passes");
-    int *mine = reinterpret_cast<int *>(lds) + wave * HT * 16 * PITCH;
+    constexpr int NP = 16 * HT / RPP, PU = NP < 8 ? NP : 8;
+    static_assert(HT0 >= 1 && TM % HT == 0 && (16 * HT) % RPP == 0 && NP % PU == 0, "whole passes");
+    asm volatile("s_barrier" ::: "memory");
+    int4_t *mine = reinterpret_cast<int4_t *>(lds) + wave * HT * 4 * PITCH;
     const int c = lane % LPR, n0 = (t0 + wn * TN) * (SWIGLU ? 8 : 16) + 8 * c;       // this lane's outputs n0 .. n0 + 7
     float s0[8], s1[8];                                                              // scales; SwiGLU: up scales, else bias
 #pragma unroll
@@ -468,54 +524,70 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
         s0[j] = a.ws[n];
         s1[j] = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
     }
-    const bool whole = n0 + 8 <= a.N, wide = whole && a.ov == 16, rwide = whole && a.rv == 16;
+    // every column of the workgroup is there and rows are 16-byte aligned (the same in all lanes)
+    const bool fast = (nt + 1) * BN <= (SWIGLU ? 2 * a.N : a.N) && a.ov == 16 && (!a.res || a.rv == 16);
+    auto outputs = [&](int row, float xs, float (&y)[8]) {
+        const int4_t *v = mine + row * (PITCH / 4);
+        if (SWIGLU) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int4_t t = v[(4 * c + q) ^ (row & CMASK)];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) y[2 * q + j] = i8_swiglu(t[j], t[2 + j], xs, s0[2 * q + j], s1[2 * q + j]);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int4_t t = v[(2 * c + q) ^ (row & CMASK)];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y[4 * q + j] = i8_scaled(t[j], xs, s0[4 * q + j], s1[4 * q + j]);
+            }
+        }
+    };
 #pragma unroll
     for (int h = 0; h < TM; h += HT) {
 #pragma unroll
         for (int i = 0; i < HT; ++i)
 #pragma unroll
-            for (int j = 0; j < TN; ++j) *reinterpret_cast<int4_t *>(mine + (16 * i + r) * PITCH + 16 * j + 4 * g) = acc[h + i][j];
+            for (int j = 0; j < TN; ++j) mine[(16 * i + r) * (PITCH / 4) + ((4 * j + g) ^ (r & CMASK))] = acc[h + i][j];
         __builtin_amdgcn_wave_barrier();
+        const int mrow = (wm * TM + h) * 16;                 // in the workgroup's tile
+        if (fast) {
 #pragma unroll 1
-        for (int p = 0; p < 16 * HT / RPP; ++p) {
-            const int row = p * RPP + lane / LPR, m = m0 + (wm * TM + h) * 16 + row;
-            const int4_t *v = reinterpret_cast<const int4_t *>(mine + row * PITCH + CP * c);
-            if (m >= a.M || n0 >= a.N) continue;
-            const float xs = a.xs[m];
-            float y[8];
-            if (SWIGLU) {
+            for (int p = 0; p < NP; p += PU) {
+                Frag rf[PU];
+                if (!SWIGLU && a.res) {
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int4_t t = v[q];
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) y[2 * q + j] = i8_swiglu(t[j], t[2 + j], xs, s0[2 * q + j], s1[2 * q + j]);
+                    for (int u = 0; u < PU; ++u)
+                        rf[u].u = *reinterpret_cast<const uint4 *>(a.res + (size_t)min(m0 + mrow + (p + u) * RPP + lane / LPR, a.M - 1) * a.ldr + n0);
                 }
-            } else {
-                const int4_t lo = v[0], hi = v[1];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    y[j] = i8_scaled(lo[j], xs, s0[j], s1[j]);
-                    y[4 + j] = i8_scaled(hi[j], xs, s0[4 + j], s1[4 + j]);
-                }
-                if (a.res) {
-                    const bf16_t *rr = a.res + (size_t)m * a.ldr + n0;
-                    Frag f;
-                    if (rwide) f.u = *reinterpret_cast<const uint4 *>(rr);
-                    else {
+                for (int u = 0; u < PU; ++u) {
+                    const int row = (p + u) * RPP + lane / LPR, m = m0 + mrow + row;
+                    float y[8];
+                    outputs(row, xscale[mrow + row], y);
+                    if (!SWIGLU && a.res) {
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) f.h[j] = n0 + j < a.N ? rr[j] : (bf16_t)0;
+                        for (int j = 0; j < 8; ++j) y[j] += bf2f(rf[u].h[j]);
                     }
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) y[j] += bf2f(f.h[j]);
+                    if (m < a.M)
+                        *reinterpret_cast<uint4 *>(a.out + (size_t)m * a.ldo + n0) =
+                            make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
                 }
             }
-            Frag f;
-            f.u = make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
-            bf16_t *o = a.out + (size_t)m * a.ldo + n0;
-            if (wide) *reinterpret_cast<uint4 *>(o) = f.u;
-            else {
+        } else {
+#pragma unroll 1
+            for (int p = 0; p < NP; ++p) {
+                const int row = p * RPP + lane / LPR, m = m0 + mrow + row;
+                if (m >= a.M || n0 >= a.N) continue;
+                float y[8];
+                outputs(row, xscale[mrow + row], y);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) if (n0 + j < a.N) o[j] = f.h[j];
+                for (int j = 0; j < 8; ++j)
+                    if (n0 + j < a.N) {
+                        if (!SWIGLU && a.res) y[j] += bf2f(a.res[(size_t)m * a.ldr + n0 + j]);
+                        a.out[(size_t)m * a.ldo + n0 + j] = f2bf(y[j]);
+                    }
             }
         }
         __builtin_amdgcn_wave_barrier();
@@ -532,8 +604,8 @@ static constexpr int g_i8_form = 0;
 
 template <bool SWIGLU>
 static void launch_form_int8(const LinI8Args &a, int tiles, int form, hipStream_t s) {
-#define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \
-        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, SWIGLU>), dim3(mt * nt), dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
+#define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST, ALT) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \
+        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, ALT, SWIGLU>), dim3(mt * nt), dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
 #define QTTS_SPLIT_I8(TM, TN, NW) hipLaunchKernelGGL((linear_int8_split_kernel<TM, TN, NW, SWIGLU>), \
         dim3(ceil_div(tiles, TN), ceil_div(a.M, 16 * TM)), dim3(NW * 64), 0, s, a)
     switch (form) {
@@ -549,21 +621,28 @@ static void launch_form_int8(const LinI8Args &a, int tiles, int form, hipStream_
     case 10: QTTS_SPLIT_I8(2, 4, 8); break;
     case 11: QTTS_SPLIT_I8(4, 4, 8); break;
     case 12: QTTS_SPLIT_I8(4, 4, 4); break;
-    case 20: QTTS_TILE_I8(64, 64, 2, 2, 1, 4); break;
-    case 21: QTTS_TILE_I8(64, 64, 2, 2, 2, 4); break;
-    case 22: QTTS_TILE_I8(64, 64, 2, 2, 2, 8); break;
-    case 23: QTTS_TILE_I8(128, 128, 2, 2, 1, 5); break;
-    case 24: QTTS_TILE_I8(128, 128, 2, 2, 2, 4); break;
-    case 25: QTTS_TILE_I8(128, 128, 2, 2, 2, 5); break;
-    case 26: QTTS_TILE_I8(256, 256, 2, 4, 1, 3); break;
-    case 27: QTTS_TILE_I8(256, 256, 2, 4, 1, 4); break;
-    case 28: QTTS_TILE_I8(256, 256, 2, 4, 1, 5); break;
-    case 29: QTTS_TILE_I8(256, 256, 4, 2, 1, 4); break;
-    case 30: QTTS_TILE_I8(256, 256, 2, 4, 2, 2); break;
-    case 31: QTTS_TILE_I8(256, 128, 4, 2, 1, 6); break;
-    case 32: QTTS_TILE_I8(128, 256, 2, 4, 1, 3); break;
-    case 33: QTTS_TILE_I8(128, 128, 2, 4, 1, 4); break;
-    case 34: QTTS_TILE_I8(128, 64, 2, 2, 2, 4); break;
+    case 20: QTTS_TILE_I8(64, 64, 2, 2, 1, 4, false); break;
+    case 21: QTTS_TILE_I8(64, 64, 2, 2, 2, 4, false); break;
+    case 22: QTTS_TILE_I8(64, 64, 2, 2, 2, 8, false); break;
+    case 23: QTTS_TILE_I8(128, 128, 2, 2, 1, 5, false); break;
+    case 24: QTTS_TILE_I8(128, 128, 2, 2, 2, 4, false); break;
+    case 25: QTTS_TILE_I8(128, 128, 2, 2, 2, 3, false); break;
+    case 26: QTTS_TILE_I8(256, 256, 2, 4, 1, 3, false); break;
+    case 27: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, false); break;
+    case 29: QTTS_TILE_I8(256, 256, 4, 2, 1, 4, false); break;
+    case 30: QTTS_TILE_I8(256, 256, 2, 4, 2, 2, false); break;
+    case 31: QTTS_TILE_I8(256, 128, 4, 2, 1, 6, false); break;
+    case 32: QTTS_TILE_I8(128, 256, 2, 4, 1, 3, false); break;
+    case 33: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, false); break;
+    case 40: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, true); break;
+    case 42: QTTS_TILE_I8(256, 256, 4, 2, 1, 4, true); break;
+    case 43: QTTS_TILE_I8(256, 256, 2, 4, 2, 2, true); break;
+    case 44: QTTS_TILE_I8(128, 256, 2, 4, 1, 4, true); break;
+    case 45: QTTS_TILE_I8(256, 128, 4, 2, 1, 4, true); break;
+    case 46: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, true); break;
+    case 47: QTTS_TILE_I8(128, 256, 2, 4, 2, 3, true); break;
+    case 48: QTTS_TILE_I8(128, 128, 2, 4, 2, 4, true); break;
+    case 34: QTTS_TILE_I8(128, 64, 2, 2, 2, 4, false); break;
     }
 #undef QTTS_TILE_I8
 #undef QTTS_SPLIT_I8
