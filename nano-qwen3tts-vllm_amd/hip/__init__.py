@@ -222,163 +222,172 @@ def linear_swiglu(x, w_gu_packed, I, norm_w=None, eps=1e-6, out=None):
 
 
 # ---- 8-bit integers: rows and weights as int8 with a scale each (a row stands for q * scale)
-def _rows_of(t, dtype, what, rows=None, cols=None, device=None):
-    """Refuses what a kernel must not be given: another device, type, shape, or rows that are not contiguous."""
-    if not t.is_cuda or t.dtype != dtype or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
-        raise QttsError(f"{what}: need [rows, columns] of {dtype} on the GPU with contiguous columns, got "
-                        f"{tuple(t.shape)} {t.dtype} on {t.device}, strides {t.stride()}")
-    if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise QttsError(f"{what}: shape {tuple(t.shape)}, need {(rows, cols)}")
-    if device is None:
-        if t.device.index != current_device():
-            raise QttsError(f"{what}: on {t.device}, but the current device is {current_device()}")
-    elif t.device != device:
-        raise QttsError(f"{what}: on {t.device}, not {device}")
+# A decode step's kernels take 3-5 us, a wrapper of torch's own checks about as long again: these read each property once.
+_raw_stream = torch._C._cuda_getCurrentRawStream       # the handle of torch.cuda.current_stream(device), without the object
 
 
-def _vector_of(t, dtype, what, n, device):
-    if not t.is_cuda or t.device != device or t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise QttsError(f"{what}: need {n} contiguous {dtype} on {device}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+def _device_of(t, what):
+    """Index of the device that all tensors of a call are on: the current one."""
+    dev = t.get_device()
+    if dev < 0 or dev != current_device():
+        raise QttsError(f"{what}: on {t.device}, need the current device" + (f", {current_device()}" if dev >= 0 else ""))
+    return dev
 
 
-def _row_stride(t):
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), t.shape[1])
+def _rows_of(t, dtype, what, dev, rows=None, cols=None):
+    """(rows, columns, row stride) of a matrix with contiguous columns."""
+    if t.get_device() != dev or t.dtype is not dtype or t.dim() != 2:
+        raise QttsError(f"{what}: need [rows, columns] of {dtype} on device {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    M, K = t.shape
+    ld, step = t.stride()
+    if step != 1 and K != 1:
+        raise QttsError(f"{what}: need contiguous columns, got strides {t.stride()}")
+    if rows is not None and (M != rows or K != cols):
+        raise QttsError(f"{what}: shape {(M, K)}, need {(rows, cols)}")
+    return M, K, ld if M > 1 or ld > K else K
+
+
+def _vector_of(t, dtype, what, dev, n):
+    if t.get_device() != dev or t.dtype is not dtype or t.shape != (n,) or (t.stride(0) != 1 and n > 1):
+        raise QttsError(f"{what}: need {n} contiguous {dtype} on device {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
+
+
+def _packed_of(t, nbytes, what, dev):
+    if t.get_device() != dev or t.dtype is not torch.uint8 or t.shape != (nbytes,):
+        raise QttsError(f"{what}: need the {nbytes} bytes that packing made for this shape, on device {dev}; got "
+                        f"{tuple(t.shape)} {t.dtype} on {t.device}")
+    return t.data_ptr()
 
 
 def int8_rows(M, K, device):
     """An int8 [M, K] buffer as the 8-bit operators take it: a row takes a multiple of 16 bytes."""
-    return torch.empty(M, (K + 15) // 16 * 16, dtype=torch.int8, device=device)[:, :K]
+    if K % 16 == 0:
+        return torch.empty((M, K), dtype=torch.int8, device=device)
+    return torch.empty((M, (K + 15) // 16 * 16), dtype=torch.int8, device=device)[:, :K]
 
 
-def _int8_stride(t, what):
-    """Row stride of int8 rows; the padding of the last row must lie inside the allocation."""
-    M, K = t.shape
-    pad = (K + 15) // 16 * 16
-    ld = t.stride(0) if M > 1 else pad
-    if pad != K and t.storage_offset() + (M - 1) * ld + pad > t.untyped_storage().nbytes():
-        raise QttsError(f"{what}: {K} columns, but a row needs {pad} readable bytes (int8_rows allocates them)")
-    return ld
+def _int8_rows_of(t, what, dev, rows=None, cols=None):
+    """_rows_of for int8 rows, whose padding to 16 bytes must lie inside the allocation, the last row's too."""
+    M, K, ld = _rows_of(t, torch.int8, what, dev, rows, cols)
+    if K % 16:
+        pad = (K + 15) // 16 * 16
+        if M == 1 and ld < pad:
+            ld = pad
+        if t.storage_offset() + (M - 1) * ld + pad > t.untyped_storage().nbytes():
+            raise QttsError(f"{what}: {K} columns, but a row needs {pad} readable bytes (int8_rows allocates them)")
+    return M, K, ld
+
+
+def _int8_out(q, scales, M, K, x, what, dev):
+    """Output rows and scales of a quantisation, made or checked: (q, its row stride, scales)."""
+    if q is None:
+        q, ldq = int8_rows(M, K, x.device), (K + 15) // 16 * 16
+    else:
+        ldq = _int8_rows_of(q, what + ": out", dev, M, K)[2]
+    if scales is None:
+        scales = torch.empty(M, dtype=torch.float32, device=x.device)
+    else:
+        _vector_of(scales, torch.float32, what + ": scales", dev, M)
+    return q, ldq, scales
 
 
 def quantize_int8(x, out=None, scales=None):
     """bf16 rows [M, K] -> (int8 [M, K], fp32 scale per row): q = rint(x / scale), scale = max(max|x| / 127, 2^-126)."""
-    _rows_of(x, torch.bfloat16, "quantize_int8: x")
-    M, K = x.shape
-    if out is None:
-        out = int8_rows(M, K, x.device)
-    else:
-        _rows_of(out, torch.int8, "quantize_int8: out", M, K, x.device)
-    if scales is None:
-        scales = torch.empty(M, dtype=torch.float32, device=x.device)
-    else:
-        _vector_of(scales, torch.float32, "quantize_int8: scales", M, x.device)
+    dev = _device_of(x, "quantize_int8: x")
+    M, K, ldx = _rows_of(x, torch.bfloat16, "quantize_int8: x", dev)
+    out, ldq, scales = _int8_out(out, scales, M, K, x, "quantize_int8", dev)
     if M:
-        check(lib.qtts_quantize_int8(x.data_ptr(), _row_stride(x), out.data_ptr(), _int8_stride(out, "quantize_int8: out"),
-                                     scales.data_ptr(), M, K, stream()), "quantize_int8")
+        check(lib.qtts_quantize_int8(x.data_ptr(), ldx, out.data_ptr(), ldq, scales.data_ptr(), M, K, _raw_stream(dev)),
+              "quantize_int8")
     return out, scales
 
 
 def rmsnorm_int8(x, w, eps=1e-6, delta=None, sum_out=None, out=None, scales=None):
     """RMSNorm(x [+ delta]) * w as int8 rows with a scale each -> (q, scales), and with delta (q, scales, bf16(x + delta)).
     sum_out may be x or delta: the sum then replaces it."""
-    _rows_of(x, torch.bfloat16, "rmsnorm_int8: x")
-    M, H = x.shape
-    dev = x.device
-    _vector_of(w, torch.bfloat16, "rmsnorm_int8: w", H, dev)
+    dev = _device_of(x, "rmsnorm_int8: x")
+    M, H, ldx = _rows_of(x, torch.bfloat16, "rmsnorm_int8: x", dev)
+    wp = _vector_of(w, torch.bfloat16, "rmsnorm_int8: w", dev, H)
+    dp = sp = None
+    ldd = lds = 0
     if delta is not None:
-        _rows_of(delta, torch.bfloat16, "rmsnorm_int8: delta", M, H, dev)
+        ldd, dp = _rows_of(delta, torch.bfloat16, "rmsnorm_int8: delta", dev, M, H)[2], delta.data_ptr()
         if sum_out is None:
-            sum_out = torch.empty(M, H, dtype=torch.bfloat16, device=dev)
+            sum_out, lds = torch.empty((M, H), dtype=torch.bfloat16, device=x.device), H
         else:
-            _rows_of(sum_out, torch.bfloat16, "rmsnorm_int8: sum_out", M, H, dev)
+            lds = _rows_of(sum_out, torch.bfloat16, "rmsnorm_int8: sum_out", dev, M, H)[2]
+        sp = sum_out.data_ptr()
     elif sum_out is not None:
         raise QttsError("rmsnorm_int8: sum_out without delta")
-    if out is None:
-        out = int8_rows(M, H, dev)
-    else:
-        _rows_of(out, torch.int8, "rmsnorm_int8: out", M, H, dev)
-    if scales is None:
-        scales = torch.empty(M, dtype=torch.float32, device=dev)
-    else:
-        _vector_of(scales, torch.float32, "rmsnorm_int8: scales", M, dev)
+    out, ldq, scales = _int8_out(out, scales, M, H, x, "rmsnorm_int8", dev)
     if M:
-        d, s = (delta, sum_out) if delta is not None else (None, None)
-        check(lib.qtts_rmsnorm_int8(x.data_ptr(), _row_stride(x), ptr(d), _row_stride(d) if d is not None else 0, w.data_ptr(),
-                                    eps, ptr(s), _row_stride(s) if s is not None else 0, out.data_ptr(),
-                                    _int8_stride(out, "rmsnorm_int8: out"), scales.data_ptr(), M, H, stream()), "rmsnorm_int8")
+        check(lib.qtts_rmsnorm_int8(x.data_ptr(), ldx, dp, ldd, wp, eps, sp, lds, out.data_ptr(), ldq, scales.data_ptr(), M, H,
+                                    _raw_stream(dev)), "rmsnorm_int8")
     return (out, scales) if delta is None else (out, scales, sum_out)
 
 
 def pack_weight_int8(w: torch.Tensor) -> torch.Tensor:
     """int8 [N, K] (quantize_int8 of a bf16 weight, or a checkpoint's) -> fragment order, as uint8."""
-    _rows_of(w, torch.int8, "pack_weight_int8: w")
-    N, K = w.shape
+    dev = _device_of(w, "pack_weight_int8: w")
+    N, K, ldw = _rows_of(w, torch.int8, "pack_weight_int8: w", dev)
     out = torch.empty(int(lib.qtts_packed_weight_int8_bytes(N, K)), dtype=torch.uint8, device=w.device)
-    check(lib.qtts_pack_weight_int8(ptr(w), _row_stride(w), ptr(out), N, K, stream()), "pack_weight_int8")
+    check(lib.qtts_pack_weight_int8(ptr(w), ldw, ptr(out), N, K, _raw_stream(dev)), "pack_weight_int8")
     return out
 
 
 def pack_gate_up_int8(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
     """int8 gate and up [I, K] -> one buffer in fragment order whose tiles hold both rows of eight outputs."""
-    _rows_of(gate, torch.int8, "pack_gate_up_int8: gate")
-    I, K = gate.shape
-    _rows_of(up, torch.int8, "pack_gate_up_int8: up", I, K, gate.device)
-    if _row_stride(gate) != _row_stride(up):
-        raise QttsError(f"pack_gate_up_int8: gate and up have row strides {_row_stride(gate)} and {_row_stride(up)}")
+    dev = _device_of(gate, "pack_gate_up_int8: gate")
+    I, K, ldw = _rows_of(gate, torch.int8, "pack_gate_up_int8: gate", dev)
+    ldu = _rows_of(up, torch.int8, "pack_gate_up_int8: up", dev, I, K)[2]
+    if ldw != ldu:
+        raise QttsError(f"pack_gate_up_int8: gate and up have row strides {ldw} and {ldu}")
     out = torch.empty(int(lib.qtts_packed_gate_up_int8_bytes(I, K)), dtype=torch.uint8, device=gate.device)
-    check(lib.qtts_pack_gate_up_int8(ptr(gate), ptr(up), _row_stride(gate), ptr(out), I, K, stream()), "pack_gate_up_int8")
+    check(lib.qtts_pack_gate_up_int8(ptr(gate), ptr(up), ldw, ptr(out), I, K, _raw_stream(dev)), "pack_gate_up_int8")
     return out
-
-
-def _packed_of(t, nbytes, what, device):
-    if t.device != device or t.dtype != torch.uint8 or t.numel() != nbytes or not t.is_contiguous():
-        raise QttsError(f"{what}: need the {nbytes} bytes that packing made for this shape, on {device}; got {t.numel()} x "
-                        f"{t.dtype} on {t.device}")
 
 
 def linear_int8(x, x_scales, w_packed, w_scales, N, bias=None, residual=None, out=None):
     """bf16(x_scales[:, None] * w_scales * (x @ w.T) + bias + residual): int8 rows x [M, K] with their scales, a weight
     [N, K] packed by pack_weight_int8 and its scale per output channel.  out may be the residual."""
-    _rows_of(x, torch.int8, "linear_int8: x")
-    M, K = x.shape
-    dev = x.device
-    _vector_of(x_scales, torch.float32, "linear_int8: x_scales", M, dev)
-    _vector_of(w_scales, torch.float32, "linear_int8: w_scales", N, dev)
-    _packed_of(w_packed, (N + 15) // 16 * ((K + 127) // 128) * 2048, "linear_int8: w_packed", dev)
+    dev = _device_of(x, "linear_int8: x")
+    M, K, ldx = _int8_rows_of(x, "linear_int8: x", dev)
+    xs = _vector_of(x_scales, torch.float32, "linear_int8: x_scales", dev, M)
+    ws = _vector_of(w_scales, torch.float32, "linear_int8: w_scales", dev, N)
+    wp = _packed_of(w_packed, (N + 15) // 16 * ((K + 127) // 128) * 2048, "linear_int8: w_packed", dev)
+    bp = rp = None
+    ldr = 0
     if bias is not None:
-        _vector_of(bias, torch.bfloat16, "linear_int8: bias", N, dev)
+        bp = _vector_of(bias, torch.bfloat16, "linear_int8: bias", dev, N)
     if residual is not None:
-        _rows_of(residual, torch.bfloat16, "linear_int8: residual", M, N, dev)
+        ldr, rp = _rows_of(residual, torch.bfloat16, "linear_int8: residual", dev, M, N)[2], residual.data_ptr()
     if out is None:
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=dev)
+        out, ldo = torch.empty((M, N), dtype=torch.bfloat16, device=x.device), N
     else:
-        _rows_of(out, torch.bfloat16, "linear_int8: out", M, N, dev)
+        ldo = _rows_of(out, torch.bfloat16, "linear_int8: out", dev, M, N)[2]
     if M:
-        check(lib.qtts_linear_int8(x.data_ptr(), _int8_stride(x, "linear_int8: x"), x_scales.data_ptr(), w_packed.data_ptr(),
-                                   w_scales.data_ptr(), ptr(bias), ptr(residual),
-                                   _row_stride(residual) if residual is not None else 0, out.data_ptr(), _row_stride(out), M, N,
-                                   K, stream()), "linear_int8")
+        check(lib.qtts_linear_int8(x.data_ptr(), ldx, xs, wp, ws, bp, rp, ldr, out.data_ptr(), ldo, M, N, K, _raw_stream(dev)),
+              "linear_int8")
     return out
 
 
 def linear_swiglu_int8(x, x_scales, w_packed, gate_scales, up_scales, I, out=None):
     """bf16(silu(g) * u) with g, u the scaled products of int8 rows x [M, K] with the gate and up rows packed by
     pack_gate_up_int8."""
-    _rows_of(x, torch.int8, "linear_swiglu_int8: x")
-    M, K = x.shape
-    dev = x.device
-    _vector_of(x_scales, torch.float32, "linear_swiglu_int8: x_scales", M, dev)
-    _vector_of(gate_scales, torch.float32, "linear_swiglu_int8: gate_scales", I, dev)
-    _vector_of(up_scales, torch.float32, "linear_swiglu_int8: up_scales", I, dev)
-    _packed_of(w_packed, (I + 7) // 8 * ((K + 127) // 128) * 2048, "linear_swiglu_int8: w_packed", dev)
+    dev = _device_of(x, "linear_swiglu_int8: x")
+    M, K, ldx = _int8_rows_of(x, "linear_swiglu_int8: x", dev)
+    xs = _vector_of(x_scales, torch.float32, "linear_swiglu_int8: x_scales", dev, M)
+    gs = _vector_of(gate_scales, torch.float32, "linear_swiglu_int8: gate_scales", dev, I)
+    us = _vector_of(up_scales, torch.float32, "linear_swiglu_int8: up_scales", dev, I)
+    wp = _packed_of(w_packed, (I + 7) // 8 * ((K + 127) // 128) * 2048, "linear_swiglu_int8: w_packed", dev)
     if out is None:
-        out = torch.empty(M, I, dtype=torch.bfloat16, device=dev)
+        out, ldo = torch.empty((M, I), dtype=torch.bfloat16, device=x.device), I
     else:
-        _rows_of(out, torch.bfloat16, "linear_swiglu_int8: out", M, I, dev)
+        ldo = _rows_of(out, torch.bfloat16, "linear_swiglu_int8: out", dev, M, I)[2]
     if M:
-        check(lib.qtts_linear_swiglu_int8(x.data_ptr(), _int8_stride(x, "linear_swiglu_int8: x"), x_scales.data_ptr(),
-                                          w_packed.data_ptr(), gate_scales.data_ptr(), up_scales.data_ptr(), out.data_ptr(),
-                                          _row_stride(out), M, I, K, stream()), "linear_swiglu_int8")
+        check(lib.qtts_linear_swiglu_int8(x.data_ptr(), ldx, xs, wp, gs, us, out.data_ptr(), ldo, M, I, K, _raw_stream(dev)),
+              "linear_swiglu_int8")
     return out
 
 
