@@ -316,14 +316,15 @@ __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int til
 union I8Frag { uint4 u; int4_t v; };
 
 // Few rows: a workgroup owns TM row tiles x TN weight tiles and its NW waves share K, each wave a contiguous run of
-// k-steps straight from memory to registers; the waves' sums meet in LDS.
-template <int TM, int TN, int NW, bool SWIGLU>
+// k-steps straight from memory to registers; the waves' sums meet in LDS.  U k-steps are requested at a time, the next U
+// before the current are multiplied.
+template <int TM, int TN, int NW, int U, bool SWIGLU>
 __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a) {
     __shared__ int4_t red[NW][TM * TN][64];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
     const int tiles = SWIGLU ? ceil_div(a.N, 8) : ceil_div(a.N, 16);
     const int t0 = blockIdx.x * TN, m0 = blockIdx.y * TM * 16;
-    const int steps = ceil_div(a.K, 64), per = ceil_div(steps, NW), ks0 = wave * per, ks1 = min(steps, ks0 + per);
+    const int steps = ceil_div(a.K, 64), per = ceil_div(steps, NW), ks0 = min(steps, wave * per), n = min(steps, ks0 + per) - ks0;
     const int8_t *xp[TM];
     const uint4 *wp[TN];
 #pragma unroll
@@ -335,17 +336,37 @@ __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a)
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < TN; ++j) acc[i][j] = int4_t{0, 0, 0, 0};
-    for (int ks = ks0; ks < ks1; ++ks) {
-        I8Frag xf[TM], wf[TN];
-        const int k = 64 * ks + 16 * g, kk = k < a.K ? k : 0;      // behind the last column the packed weights are zeros
+    struct Batch { I8Frag x[U][TM], w[U][TN]; } b0, b1;
+    auto request = [&](Batch &b, int at) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) xf[i].u = *reinterpret_cast<const uint4 *>(xp[i] + kk);
+        for (int u = 0; u < U; ++u) {
+            const int ks = ks0 + min(at + u, n - 1);                                // behind the run: its last step again, not multiplied
+            const int k = 64 * ks + 16 * g, kk = k < a.K ? k : 0;                    // behind the last column the packed weights are zeros
 #pragma unroll
-        for (int i = 0; i < TN; ++i) wf[i].u = wp[i][(size_t)ks * 64];
+            for (int i = 0; i < TM; ++i) b.x[u][i].u = *reinterpret_cast<const uint4 *>(xp[i] + kk);
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
+            for (int i = 0; i < TN; ++i) b.w[u][i].u = wp[i][(size_t)ks * 64];
+        }
+    };
+    auto multiply = [&](const Batch &b, int at) {
 #pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
+        for (int u = 0; u < U; ++u) {
+            if (at + u >= n) break;
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.w[u][j].v, b.x[u][i].v, acc[i][j], 0, 0, 0);
+        }
+    };
+    if (n > 0) {
+        request(b0, 0);
+        for (int at = 0; at < n; at += 2 * U) {
+            if (at + U < n) request(b1, at + U);
+            multiply(b0, at);
+            if (at + U >= n) break;
+            if (at + 2 * U < n) request(b0, at + 2 * U);
+            multiply(b1, at + U);
+        }
     }
 #pragma unroll
     for (int i = 0; i < TM; ++i)
@@ -353,9 +374,11 @@ __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a)
         for (int j = 0; j < TN; ++j) red[wave][i * TN + j][lane] = acc[i][j];
     __syncthreads();
     for (int t = wave; t < TM * TN; t += NW) {
-        int4_t sum = red[0][t][lane];
+        int4_t part[NW], sum = {0, 0, 0, 0};
 #pragma unroll
-        for (int w = 1; w < NW; ++w) sum += red[w][t][lane];
+        for (int w = 0; w < NW; ++w) part[w] = red[w][t][lane];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) sum += part[w];
         if (t0 + t % TN < tiles) i8_store<SWIGLU>(a, sum, t0 + t % TN, m0 + 16 * (t / TN) + r, lane);
     }
 }
@@ -391,34 +414,67 @@ __device__ __forceinline__ void wait_and_meet() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
+// What a lane needs of the outputs it stores: scale (SwiGLU: of the gate) and bias (SwiGLU: the up rows' scale) of its
+// columns, and the row scales of its wave's rows, one row per lane and word.
+template <int XW, int OUT>
+struct I8Tail {
+    float s0[OUT], s1[OUT], xs[XW];
+    __device__ __forceinline__ void arrived() const {          // the loads' wait goes here, in front of what follows in assembly
+#pragma unroll
+        for (int j = 0; j < OUT; ++j) asm volatile("" ::"v"(s0[j]), "v"(s1[j]));
+#pragma unroll
+        for (int j = 0; j < XW; ++j) asm volatile("" ::"v"(xs[j]));
+    }
+};
+
 template <int BM, int BN, int WM, int WN, int KS, int ST, bool ALT, bool SWIGLU>
 __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Args a, int mtiles, int ntiles) {
     constexpr int NW = WM * WN, RPR = 16 / KS, CPR = 4 * KS;       // rows of a request, 16-byte chunks of a row
     constexpr int NA = BM / RPR / NW, NB = BN / 16 * KS / NW, TM = BM / WM / 16, TN = BN / WN / 16;
     constexpr int STAGE = (BM + BN) * CPR;                         // 16-byte places of a stage
+    constexpr int WAIT = (ST - 2) * (NA + NB);
     static_assert(BM % (RPR * NW) == 0 && (BN / 16 * KS) % NW == 0 && (RPR * NW) % 16 == 0, "whole requests per wave");
-    static_assert((ST - 2) * (NA + NB) <= 63, "the wait counter's range");
-    __shared__ uint4 lds[ST * STAGE];
-    __shared__ float xscale[BM];
+    static_assert(WAIT <= 63, "the wait counter's range");
+    // the epilogue: a lane's OUT outputs come from CP sums; LPR lanes to a row, RPP rows a pass; HT row tiles turned at a time,
+    // in the last stage's place where that holds a row tile of every wave, otherwise behind the stages
+    constexpr int OUT = SWIGLU && TN < 4 ? 4 : 8, CP = SWIGLU ? 2 * OUT : OUT;
+    constexpr int LPR = TN * 16 / CP, RPP = 64 / LPR, CMASK = (TN * 4 < 16 ? TN * 4 : 16) - 1;
+    constexpr int ROWTILE = NW * 64 * TN;                          // places of one row tile of every wave
+    constexpr bool OVER = STAGE >= ROWTILE;
+    constexpr int HT0 = OVER ? STAGE / ROWTILE : 1, HT = HT0 >= TM ? TM : HT0 >= 4 && TM % 4 == 0 ? 4 : HT0 >= 2 && TM % 2 == 0 ? 2 : 1;
+    constexpr int NP = 16 * HT / RPP, XW = (TM * 16 + 63) / 64;
+    static_assert(TM % HT == 0 && (16 * HT) % RPP == 0, "whole passes");
+    constexpr int PLACES = ST * STAGE + (OVER ? 0 : ROWTILE);
+    static_assert(PLACES <= 10240, "160 KB of LDS");
+    __shared__ uint4 lds[PLACES];
+
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int id = blockIdx.x;
-    const int total = mtiles * ntiles;
-    if (total % 8 == 0) id = (id & 7) * (total >> 3) + (id >> 3);      // workgroups are dealt to the 8 XCDs in turn
-    const int mt = id / ntiles, nt = id % ntiles;
-    const int m0 = mt * BM, t0 = nt * (BN / 16);
+    const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
     const int tiles = SWIGLU ? ceil_div(a.N, 8) : ceil_div(a.N, 16);
-    for (int i = threadIdx.x; i < BM; i += NW * 64) xscale[i] = a.xs[min(m0 + i, a.M - 1)];
-    const int8_t *xp[NA];
-    const int rr = lane / CPR, chunk = (lane % CPR) ^ i8_swizzle<KS>(RPR * wave + rr);
-#pragma unroll
-    for (int i = 0; i < NA; ++i) xp[i] = a.x + (size_t)min(m0 + RPR * (wave + i * NW) + rr, a.M - 1) * a.ldx;
-    const uint4 *wp[NB];
-#pragma unroll
-    for (int i = 0; i < NB; ++i) {
-        const int v = wave + i * NW;
-        wp[i] = a.wp + ((size_t)min(t0 + v / KS, tiles - 1) * a.ksteps + v % KS) * 64 + lane;
-    }
+    const int nk = a.ksteps / KS, total = mtiles * ntiles;
     const uint32_t lds_at = lds_address(lds) + wave * 1024;
+    const int rr = lane / CPR, chunk = (lane % CPR) ^ i8_swizzle<KS>(RPR * wave + rr);
+    const int xat = (wm * TM * 16 + r) * CPR + (g ^ i8_swizzle<KS>(r)), wat = BM * CPR + wn * TN * 64 * KS + lane;
+
+    // the tile whose requests go out
+    int m0, t0;
+    const int8_t *xp[NA];
+    const uint4 *wp[NB];
+    auto place = [&](int b) {
+        // Workgroups are dealt to the 8 XCDs in turn: an XCD takes a run of tiles that lie together, four row blocks wide, so that
+        // its workgroups share rows and weights in its L2.
+        const int xcd = b & 7, each = total >> 3, id = xcd * each + min(xcd, total & 7) + (b >> 3);
+        const int band = id / (4 * ntiles), in = id - band * 4 * ntiles, rows = min(4, mtiles - 4 * band);
+        m0 = (4 * band + in % rows) * BM;
+        t0 = in / rows * (BN / 16);
+#pragma unroll
+        for (int i = 0; i < NA; ++i) xp[i] = a.x + (size_t)min(m0 + RPR * (wave + i * NW) + rr, a.M - 1) * a.ldx;
+#pragma unroll
+        for (int i = 0; i < NB; ++i) {
+            const int v = wave + i * NW;
+            wp[i] = a.wp + ((size_t)min(t0 + v / KS, tiles - 1) * a.ksteps + v % KS) * 64 + lane;
+        }
+    };
     auto request = [&](int it, int stage) {
         const int k = 64 * KS * it + 16 * chunk, kk = k < a.K ? k : 0;
         const uint32_t to = lds_at + stage * (STAGE * 16);
@@ -427,170 +483,208 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 #pragma unroll
         for (int i = 0; i < NB; ++i) lds_request16(wp[i] + (size_t)it * (64 * KS), to + BM * CPR * 16 + i * NW * 1024);
     };
-    const int wm = wave / WN, wn = wave % WN, r = lane & 15, g = lane >> 4;
-    const int xat = (wm * TM * 16 + r) * CPR + (g ^ i8_swizzle<KS>(r)), wat = BM * CPR + wn * TN * 64 * KS + lane;
-    int4_t acc[TM][TN];
+    auto begin = [&] {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = int4_t{0, 0, 0, 0};
-    const int nk = a.ksteps / KS;
-#pragma unroll
-    for (int i = 0; i < ST - 1; ++i) if (i < nk) request(i, i);
-    int stage = 0, next = ST - 1;
-    if (!ALT) {
-        for (int it = 0; it < nk; ++it) {
-            if (it + ST - 2 < nk) wait_and_meet<(ST - 2) * (NA + NB)>();
-            else wait_and_meet<0>();
-            if (it + ST - 1 < nk) request(it + ST - 1, next);
-            const uint4 *st = lds + stage * STAGE;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                I8Frag xf[TM], wf[TN];
-#pragma unroll
-                for (int j = 0; j < TN; ++j) wf[j].u = st[wat + j * 64 * KS + s * 64];
-#pragma unroll
-                for (int i = 0; i < TM; ++i) xf[i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
-            }
-            stage = stage + 1 == ST ? 0 : stage + 1;
-            next = next + 1 == ST ? 0 : next + 1;
-        }
-    } else {
-        // The two waves of a SIMD take turns: while one multiplies, the other reads its fragments of the next k-step, and a
-        // barrier after each turn keeps them so.  Turns: waves 0-3 read step k in turn 2k and multiply it in turn 2k + 1, waves
-        // 4-7 one turn later.  Stage k is complete before turn 2k: every wave waits for its own requests of it at the end of
-        // turn 2k - 1.  Requests into the place of stage k - 1, last read in turn 2k - 1, go out from turn 2k on.
-        const bool late = wave >= NW / 2;
-        if (ST - 1 <= nk) wait_and_meet<(ST - 2) * (NA + NB)>();
-        else wait_and_meet<0>();
-        if (late) asm volatile("s_barrier" ::: "memory");
-        for (int it = 0; it < nk; ++it) {
-            I8Frag xf[KS][TM], wf[KS][TN];
-            const uint4 *st = lds + stage * STAGE;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-#pragma unroll
-                for (int j = 0; j < TN; ++j) wf[s][j].u = st[wat + j * 64 * KS + s * 64];
-#pragma unroll
-                for (int i = 0; i < TM; ++i) xf[s][i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
-            }
-            const bool more = it + ST - 1 < nk;
-            if (more) request(it + ST - 1, next);
-            __builtin_amdgcn_sched_barrier(0);
-            if (late) {
-                if (more) wait_and_meet<(ST - 2) * (NA + NB)>();
-                else wait_and_meet<0>();
-            } else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int i = 0; i < TM; ++i)
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[s][j].v, xf[s][i].v, acc[i][j], 0, 0, 0);
-            __builtin_amdgcn_s_setprio(0);
-            __builtin_amdgcn_sched_barrier(0);
-            if (!late) {
-                if (more) wait_and_meet<(ST - 2) * (NA + NB)>();
-                else wait_and_meet<0>();
-            } else asm volatile("s_barrier" ::: "memory");
-            __builtin_amdgcn_sched_barrier(0);
-            stage = stage + 1 == ST ? 0 : stage + 1;
-            next = next + 1 == ST ? 0 : next + 1;
-        }
-        if (!late) asm volatile("s_barrier" ::: "memory");
-    }
-    // Epilogue.  A wave turns its sums round in LDS of its own, HT row tiles at a time, so that a lane has eight neighbouring
-    // outputs of a row: 16-byte loads and stores, and the same columns - hence the same scales and bias, in registers - in
-    // every pass.  The passes stay a loop, PU of them at a time so that their residual rows are requested together: unrolled over
-    // the tile's sums the epilogue was 48 KB of code, fetched once per workgroup, and took 13 us of a 49 us launch.
-    // The 16-byte chunk c of row r lies at place c ^ r (modulo the chunks of a row, 16 at most).
-    constexpr int CP = SWIGLU ? 16 : 8, LPR = TN * 16 / CP, PITCH = TN * 16, RPP = 64 / LPR, CMASK = (TN * 4 < 16 ? TN * 4 : 16) - 1;
-    constexpr int HT0 = ST * STAGE * 4 / (NW * 16 * PITCH), HT = HT0 >= TM ? TM : HT0 >= 4 && TM % 4 == 0 ? 4 : HT0 >= 2 && TM % 2 == 0 ? 2 : 1;
-    constexpr int NP = 16 * HT / RPP, PU = NP < 8 ? NP : 8;
-    static_assert(HT0 >= 1 && TM % HT == 0 && (16 * HT) % RPP == 0 && NP % PU == 0, "whole passes");
-    asm volatile("s_barrier" ::: "memory");
-    int4_t *mine = reinterpret_cast<int4_t *>(lds) + wave * HT * 4 * PITCH;
-    const int c = lane % LPR, n0 = (t0 + wn * TN) * (SWIGLU ? 8 : 16) + 8 * c;       // this lane's outputs n0 .. n0 + 7
-    float s0[8], s1[8];                                                              // scales; SwiGLU: up scales, else bias
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const int n = min(n0 + j, a.N - 1);
-        s0[j] = a.ws[n];
-        s1[j] = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
-    }
-    // every column of the workgroup is there and rows are 16-byte aligned (the same in all lanes)
-    const bool fast = (nt + 1) * BN <= (SWIGLU ? 2 * a.N : a.N) && a.ov == 16 && (!a.res || a.rv == 16);
-    auto outputs = [&](int row, float xs, float (&y)[8]) {
-        const int4_t *v = mine + row * (PITCH / 4);
-        if (SWIGLU) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int4_t t = v[(4 * c + q) ^ (row & CMASK)];
-#pragma unroll
-                for (int j = 0; j < 2; ++j) y[2 * q + j] = i8_swiglu(t[j], t[2 + j], xs, s0[2 * q + j], s1[2 * q + j]);
-            }
-        } else {
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int4_t t = v[(2 * c + q) ^ (row & CMASK)];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y[4 * q + j] = i8_scaled(t[j], xs, s0[4 * q + j], s1[4 * q + j]);
-            }
-        }
+        for (int i = 0; i < ST - 1; ++i) if (i < nk) request(i, i);
     };
+
+    // Requests return in the order they were made, stores among them.  Behind an epilogue whose stores are known to be STORES
+    // instructions of this wave, they may be under way still while the stages requested before them are waited for.
+    constexpr int STORES = TM / HT * NP;                           // one a pass
+    static_assert(WAIT + STORES <= 63, "the wait counter's range");
+    int loose = 0;                                                 // stages requested before those stores
+    auto meet = [&](int it) {                                      // stage `it` is complete, in every wave
+        if (it < min(loose, nk - ST + 2)) wait_and_meet<WAIT + STORES>();
+        else if (it < nk - ST + 2) wait_and_meet<WAIT>();
+        else wait_and_meet<0>();
+    };
+    int4_t acc[TM][TN];
+    place(blockIdx.x);
+    begin();
+    for (int b = blockIdx.x; b < total; b += gridDim.x) {
 #pragma unroll
-    for (int h = 0; h < TM; h += HT) {
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int i = 0; i < HT; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) mine[(16 * i + r) * (PITCH / 4) + ((4 * j + g) ^ (r & CMASK))] = acc[h + i][j];
-        __builtin_amdgcn_wave_barrier();
-        const int mrow = (wm * TM + h) * 16;                 // in the workgroup's tile
-        if (fast) {
+            for (int j = 0; j < TN; ++j) acc[i][j] = int4_t{0, 0, 0, 0};
+        int stage = 0, next = ST - 1;
+        if (!ALT) {
 #pragma unroll 1
-            for (int p = 0; p < NP; p += PU) {
-                Frag rf[PU];
-                if (!SWIGLU && a.res) {
+            for (int it = 0; it < nk; ++it) {
+                meet(it);
+                if (it + ST - 1 < nk) request(it + ST - 1, next);
+                const uint4 *st = lds + stage * STAGE;
 #pragma unroll
-                    for (int u = 0; u < PU; ++u)
-                        rf[u].u = *reinterpret_cast<const uint4 *>(a.res + (size_t)min(m0 + mrow + (p + u) * RPP + lane / LPR, a.M - 1) * a.ldr + n0);
+                for (int s = 0; s < KS; ++s) {
+                    I8Frag xf[TM], wf[TN];
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) wf[j].u = st[wat + j * 64 * KS + s * 64];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) xf[i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[j].v, xf[i].v, acc[i][j], 0, 0, 0);
                 }
-#pragma unroll
-                for (int u = 0; u < PU; ++u) {
-                    const int row = (p + u) * RPP + lane / LPR, m = m0 + mrow + row;
-                    float y[8];
-                    outputs(row, xscale[mrow + row], y);
-                    if (!SWIGLU && a.res) {
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) y[j] += bf2f(rf[u].h[j]);
-                    }
-                    if (m < a.M)
-                        *reinterpret_cast<uint4 *>(a.out + (size_t)m * a.ldo + n0) =
-                            make_uint4(pack2(y[0], y[1]), pack2(y[2], y[3]), pack2(y[4], y[5]), pack2(y[6], y[7]));
-                }
+                stage = stage + 1 == ST ? 0 : stage + 1;
+                next = next + 1 == ST ? 0 : next + 1;
             }
+            wait_and_meet<0>();
         } else {
+            // The two waves of a SIMD take turns: while one multiplies, the other reads its fragments of the next k-step, and a
+            // barrier after each turn keeps them so.  Turns: waves 0-3 read step k in turn 2k and multiply it in turn 2k + 1,
+            // waves 4-7 one turn later.  Stage k is complete before turn 2k: every wave waits for its own requests of it at the
+            // end of turn 2k - 1.  Requests into the place of stage k - 1, last read in turn 2k - 1, go out from turn 2k on.
+            const bool late = wave >= NW / 2;
+            meet(0);
+            if (late) asm volatile("s_barrier" ::: "memory");
 #pragma unroll 1
-            for (int p = 0; p < NP; ++p) {
-                const int row = p * RPP + lane / LPR, m = m0 + mrow + row;
-                if (m >= a.M || n0 >= a.N) continue;
-                float y[8];
-                outputs(row, xscale[mrow + row], y);
+            for (int it = 0; it < nk; ++it) {
+                I8Frag xf[KS][TM], wf[KS][TN];
+                const uint4 *st = lds + stage * STAGE;
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    if (n0 + j < a.N) {
-                        if (!SWIGLU && a.res) y[j] += bf2f(a.res[(size_t)m * a.ldr + n0 + j]);
-                        a.out[(size_t)m * a.ldo + n0 + j] = f2bf(y[j]);
-                    }
+                for (int s = 0; s < KS; ++s) {
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) wf[s][j].u = st[wat + j * 64 * KS + s * 64];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) xf[s][i].u = st[(xat ^ (4 * s)) + i * 16 * CPR];
+                }
+                if (it + ST - 1 < nk) request(it + ST - 1, next);
+                __builtin_amdgcn_sched_barrier(0);
+                if (late) meet(it + 1);
+                else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[s][j].v, xf[s][i].v, acc[i][j], 0, 0, 0);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                if (!late) meet(it + 1);
+                else asm volatile("s_barrier" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+                stage = stage + 1 == ST ? 0 : stage + 1;
+                next = next + 1 == ST ? 0 : next + 1;
             }
+            if (!late) asm volatile("s_barrier" ::: "memory");
         }
-        __builtin_amdgcn_wave_barrier();
+        // Every read of the stages is done (the barriers above).  The next tile's first ST - 1 stages are requested now and come
+        // in under the epilogue, which turns the sums round in the last stage's place.
+        // What the epilogue needs of the scales is waited for before that: requests return in order.
+        const int row0 = m0 + wm * TM * 16, nw = (t0 + wn * TN) * (SWIGLU ? 8 : 16), n0 = nw + OUT * (lane % LPR);
+        I8Tail<XW, OUT> now;
+#pragma unroll
+        for (int j = 0; j < OUT; ++j) {
+            const int n = min(n0 + j, a.N - 1);
+            now.s0[j] = a.ws[n];
+            now.s1[j] = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < XW; ++j) now.xs[j] = a.xs[min(row0 + 64 * j + lane, a.M - 1)];
+        const bool wide = a.N % OUT == 0 && a.ov >= 2 * OUT && (SWIGLU || !a.res || a.rv == 16);      // whole pieces, aligned
+        // Residual rows are requested RB passes ahead.  Behind the last row the last is read: the loads stay unconditional.
+        constexpr int PASSES = TM / HT * NP, RB = SWIGLU ? 1 : PASSES < 8 ? PASSES : 8;
+        u32x4_t rf[RB];
+        const bool add = !SWIGLU && wide && a.res;
+        auto residual = [&](int pass) {
+            return *reinterpret_cast<const u32x4_t *>(a.res + (size_t)min(row0 + lane / LPR + pass * RPP, a.M - 1) * a.ldr + min(n0, a.N - OUT));
+        };
+        if (add) {
+#pragma unroll
+            for (int p = 0; p < RB; ++p) rf[p] = residual(p);
+#pragma unroll
+            for (int p = 0; p < RB; ++p) asm volatile("" ::"v"(rf[p]));
+        }
+        now.arrived();
+        if (b + (int)gridDim.x < total) {
+            place(b + gridDim.x);
+            begin();
+        }
+        // Epilogue.  A wave turns its sums round in LDS of its own, HT row tiles at a time, so that a lane has neighbouring
+        // outputs of a row: 16-byte loads and stores, and the same columns - hence the same scales and bias, in registers - in
+        // every pass.  The 16-byte chunk c of row q lies at place c ^ q (modulo the chunks of a row, 16 at most).
+        int4_t *mine = reinterpret_cast<int4_t *>(lds + (OVER ? ST - 1 : ST) * STAGE) + wave * HT * 64 * TN;
+        const int lrow = lane / LPR, c = lane % LPR;
+        auto outputs = [&](int pass, float xs, float (&y)[OUT]) {
+            const int4_t *v = mine + (pass * RPP + lrow) * (TN * 4);
+            const int turn = (lrow & CMASK) ^ ((pass * RPP) & CMASK);
+            if (SWIGLU) {
+#pragma unroll
+                for (int q = 0; q < OUT / 2; ++q) {
+                    const int4_t t = v[(OUT / 2 * c + q) ^ turn];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) y[2 * q + j] = i8_swiglu(t[j], t[2 + j], xs, now.s0[2 * q + j], now.s1[2 * q + j]);
+                }
+            } else {
+#pragma unroll
+                for (int q = 0; q < OUT / 4; ++q) {
+                    const int4_t t = v[(OUT / 4 * c + q) ^ turn];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) y[4 * q + j] = i8_scaled(t[j], xs, now.s0[4 * q + j], now.s1[4 * q + j]);
+                }
+            }
+        };
+        auto row_scale = [&](int row) { return __shfl(now.xs[row >> 6], (row & 63) + lrow); };    // row: a constant, a multiple of RPP
+        const int have = n0 < a.N ? a.M - row0 - lrow : 0;      // rows from this lane's first on
+        bf16_t *op = a.out + (size_t)(row0 + lrow) * a.ldo + n0;
+        const size_t ostep = (size_t)RPP * a.ldo;
+        // every pass stores something: the rows are there, and the wave's first column
+        loose = wide && row0 + TM * 16 <= a.M && nw < a.N ? ST - 1 : 0;
+#pragma unroll
+        for (int h = 0; h < TM; h += HT) {
+#pragma unroll
+            for (int i = 0; i < HT; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) mine[(16 * i + r) * (TN * 4) + ((4 * j + g) ^ (r & CMASK))] = acc[h + i][j];
+            __builtin_amdgcn_wave_barrier();
+            if (wide) {
+#pragma unroll
+                for (int p = 0; p < NP; ++p) {
+                    float y[OUT];
+                    outputs(p, row_scale(h * 16 + p * RPP), y);
+                    if (add) {
+                        const int pass = h / HT * NP + p;
+#pragma unroll
+                        for (int j = 0; j < OUT; j += 2) {
+                            float lo, hi;
+                            unpack2(rf[pass % RB][j / 2], lo, hi);
+                            y[j] += lo;
+                            y[j + 1] += hi;
+                        }
+                        if (pass + RB < PASSES) rf[pass % RB] = residual(pass + RB);
+                    }
+                    uint32_t packed[OUT / 2];
+#pragma unroll
+                    for (int j = 0; j < OUT; j += 2) packed[j / 2] = pack2v(float2_t{y[j], y[j + 1]});
+                    if (h * 16 + p * RPP < have) {
+                        if constexpr (OUT == 8) *reinterpret_cast<uint4 *>(op) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
+                        else *reinterpret_cast<uint2 *>(op) = make_uint2(packed[0], packed[1]);
+                    }
+                    op += ostep;
+                }
+            } else {
+                // the last columns, or rows that are not aligned: an output at a time, neighbouring lanes neighbouring columns
+                constexpr int COLS = TN * (SWIGLU ? 8 : 16);
+                const int *flat = reinterpret_cast<const int *>(mine);
+#pragma unroll 4
+                for (int e = lane; e < 16 * HT * COLS; e += 64) {
+                    const int row = e / COLS, col = e % COLS, m = min(row0 + h * 16 + row, a.M - 1), n = min(nw + col, a.N - 1);
+                    const int pc = SWIGLU ? (col >> 1) * 4 + (col & 1) : col;          // packed column of the sum (of the gate's)
+                    const int at = (row * (TN * 4) + ((pc >> 2) ^ (row & CMASK))) * 4 + (pc & 3);
+                    float y;
+                    if (SWIGLU) y = i8_swiglu(flat[at], flat[at + 2], a.xs[m], a.ws[n], a.us[n]);
+                    else {
+                        y = i8_scaled(flat[at], a.xs[m], a.ws[n], a.bias ? bf2f(a.bias[n]) : 0.f);
+                        if (a.res) y += bf2f(a.res[(size_t)m * a.ldr + n]);
+                    }
+                    if (row0 + h * 16 + row < a.M && nw + col < a.N) a.out[(size_t)m * a.ldo + n] = f2bf(y);
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
 
@@ -605,23 +699,29 @@ static constexpr int g_i8_form = 0;
 template <bool SWIGLU>
 static void launch_form_int8(const LinI8Args &a, int tiles, int form, hipStream_t s) {
 #define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST, ALT) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \
-        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, ALT, SWIGLU>), dim3(mt * nt), dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
-#define QTTS_SPLIT_I8(TM, TN, NW) hipLaunchKernelGGL((linear_int8_split_kernel<TM, TN, NW, SWIGLU>), \
+        constexpr int PER_CU = 163840 / (ST * (BM + BN) * KS * 64) > 0 ? 163840 / (ST * (BM + BN) * KS * 64) : 1; \
+        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, ALT, SWIGLU>), dim3(std::min(mt * nt, 256 * PER_CU)), dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
+#define QTTS_SPLIT_I8(TM, TN, NW, U) hipLaunchKernelGGL((linear_int8_split_kernel<TM, TN, NW, U, SWIGLU>), \
         dim3(ceil_div(tiles, TN), ceil_div(a.M, 16 * TM)), dim3(NW * 64), 0, s, a)
     switch (form) {
-    case 1: QTTS_SPLIT_I8(1, 1, 4); break;
-    case 2: QTTS_SPLIT_I8(1, 1, 8); break;
-    case 3: QTTS_SPLIT_I8(1, 2, 8); break;
-    case 4: QTTS_SPLIT_I8(2, 1, 8); break;
-    case 5: QTTS_SPLIT_I8(2, 2, 8); break;
-    case 6: QTTS_SPLIT_I8(4, 1, 8); break;
-    case 7: QTTS_SPLIT_I8(4, 2, 8); break;
-    case 8: QTTS_SPLIT_I8(2, 2, 4); break;
-    case 9: QTTS_SPLIT_I8(4, 2, 4); break;
-    case 10: QTTS_SPLIT_I8(2, 4, 8); break;
-    case 11: QTTS_SPLIT_I8(4, 4, 8); break;
-    case 12: QTTS_SPLIT_I8(4, 4, 4); break;
-    case 20: QTTS_TILE_I8(64, 64, 2, 2, 1, 4, false); break;
+    case 1: QTTS_SPLIT_I8(1, 1, 4, 4); break;
+    case 2: QTTS_SPLIT_I8(1, 1, 8, 4); break;
+    case 3: QTTS_SPLIT_I8(1, 2, 8, 4); break;
+    case 4: QTTS_SPLIT_I8(2, 1, 8, 4); break;
+    case 5: QTTS_SPLIT_I8(2, 2, 8, 2); break;
+    case 6: QTTS_SPLIT_I8(2, 2, 8, 4); break;
+    case 7: QTTS_SPLIT_I8(4, 2, 8, 2); break;
+    case 8: QTTS_SPLIT_I8(2, 2, 4, 4); break;
+    case 9: QTTS_SPLIT_I8(4, 2, 4, 2); break;
+    case 10: QTTS_SPLIT_I8(2, 4, 8, 2); break;
+    case 11: QTTS_SPLIT_I8(4, 4, 8, 2); break;
+    case 12: QTTS_SPLIT_I8(4, 4, 4, 2); break;
+    case 13: QTTS_SPLIT_I8(1, 1, 16, 4); break;
+    case 14: QTTS_SPLIT_I8(1, 2, 4, 4); break;
+    case 15: QTTS_SPLIT_I8(1, 1, 16, 2); break;
+    case 16: QTTS_SPLIT_I8(1, 1, 8, 6); break;
+    case 17: QTTS_SPLIT_I8(2, 4, 4, 2); break;
+    case 18: QTTS_SPLIT_I8(4, 4, 8, 1); break;
     case 21: QTTS_TILE_I8(64, 64, 2, 2, 2, 4, false); break;
     case 22: QTTS_TILE_I8(64, 64, 2, 2, 2, 8, false); break;
     case 23: QTTS_TILE_I8(128, 128, 2, 2, 1, 5, false); break;
@@ -629,13 +729,13 @@ static void launch_form_int8(const LinI8Args &a, int tiles, int form, hipStream_
     case 25: QTTS_TILE_I8(128, 128, 2, 2, 2, 3, false); break;
     case 26: QTTS_TILE_I8(256, 256, 2, 4, 1, 3, false); break;
     case 27: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, false); break;
-    case 29: QTTS_TILE_I8(256, 256, 4, 2, 1, 4, false); break;
+    case 29: QTTS_TILE_I8(256, 256, 4, 2, 1, 3, false); break;
     case 30: QTTS_TILE_I8(256, 256, 2, 4, 2, 2, false); break;
-    case 31: QTTS_TILE_I8(256, 128, 4, 2, 1, 6, false); break;
+    case 31: QTTS_TILE_I8(256, 128, 4, 2, 1, 5, false); break;
     case 32: QTTS_TILE_I8(128, 256, 2, 4, 1, 3, false); break;
     case 33: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, false); break;
     case 40: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, true); break;
-    case 42: QTTS_TILE_I8(256, 256, 4, 2, 1, 4, true); break;
+    case 42: QTTS_TILE_I8(256, 256, 4, 2, 1, 3, true); break;
     case 43: QTTS_TILE_I8(256, 256, 2, 4, 2, 2, true); break;
     case 44: QTTS_TILE_I8(128, 256, 2, 4, 1, 4, true); break;
     case 45: QTTS_TILE_I8(256, 128, 4, 2, 1, 4, true); break;
