@@ -688,74 +688,74 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
     }
 }
 
-// The forms a product may take, by number (a measurement build may force one: qtts_tune_int8)
+// ---- which form a product takes
+// A workgroup's time is a fixed part and a part per k-step, the bytes its CU pulls in at 50-70 GB/s (few bytes: latency); a
+// launch's is that times the workgroups a CU gets, on top of what the launch itself takes:
+//   us = launch + (fixed + step * ceil(K / 64)) * load,   load = max(1, r + 3/4 (ceil(r) - r)),  r = workgroups / 256
+// fitted to the times of every form over 1-8192 rows and nine N x K from 1024 x 1024 to 8192 x 512 (cold weights, in a graph).
+// The form with the smallest estimate is taken: over those 261 shapes 0.8 % slower on average than the fastest form of each, at
+// most 14 %.  Some of them (us of the forms in the table's order, '-' far off):
+//   1 x 4096 x 2048 (plain)       3.9  3.9  4.2  4.8  5.5  6.8   -    -    -    -
+//   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   16   -    -    -    -
+//   200 x 4096 x 2048 (plain)      17   17   12   12   11  7.9   13   13   17   26
+//   800 x 4096 x 2048 (plain)       -    -    -    -    -   20   15   14   18   29
+//   4096 x 4096 x 2048 (plain)      -    -    -    -    -   65   44   50   41   38
+struct I8Form { int bm, bn; float launch, fixed, step; };
+static constexpr I8Form I8_FORMS[] = {
+    {16, 16, 2.52f, 0.117f, 0.037f},     // K over 4 waves
+    {16, 16, 2.37f, 0.448f, 0.031f},     // over 8
+    {16, 32, 2.42f, 0.147f, 0.048f},     // over 4
+    {32, 32, 2.04f, 0.565f, 0.073f},     // over 8
+    {32, 64, 1.84f, 1.029f, 0.109f},     // over 8
+    {64, 64, 3.50f, 0.409f, 0.112f},     // through LDS, as the rest
+    {128, 128, 3.97f, 1.346f, 0.279f},
+    {128, 128, 1.57f, 3.497f, 0.280f},   // two k-steps a stage, waves in turns
+    {128, 256, 0.94f, 6.138f, 0.387f},   // the same
+    {256, 256, 0.04f, 11.115f, 0.670f},  // one k-step a stage, waves in turns
+};
+static constexpr int I8_SPLIT_FORMS = 5;
 #ifdef QTTS_TUNING
-static int g_i8_form = 0;
-extern "C" void qtts_tune_int8(int form) { g_i8_form = form; }
+static int g_i8_form = -1;
+extern "C" void qtts_tune_int8(int form) { g_i8_form = form; }      // measurement builds: this form whatever the shape
 #else
-static constexpr int g_i8_form = 0;
+static constexpr int g_i8_form = -1;
 #endif
 
+static int choose_int8_form(int M, int columns, int K) {
+    if (g_i8_form >= 0) return g_i8_form;
+    int best = -1;
+    double least = 0;
+    for (int f = 0; f < (int)(sizeof(I8_FORMS) / sizeof(I8_FORMS[0])); ++f) {
+        const I8Form &F = I8_FORMS[f];
+        if (f < I8_SPLIT_FORMS && ceil_div(M, F.bm) > 65535) continue;              // the row blocks are blockIdx.y there
+        const double r = (double)ceil_div(M, F.bm) * ceil_div(columns, F.bn) / 256;
+        const double us = F.launch + (F.fixed + F.step * ceil_div(K, 64)) * std::max(1.0, 0.25 * r + 0.75 * ceil(r));
+        if (best < 0 || us < least) { best = f; least = us; }
+    }
+    return best;
+}
+
 template <bool SWIGLU>
-static void launch_form_int8(const LinI8Args &a, int tiles, int form, hipStream_t s) {
-#define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST, ALT) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \
-        constexpr int PER_CU = 163840 / (ST * (BM + BN) * KS * 64) > 0 ? 163840 / (ST * (BM + BN) * KS * 64) : 1; \
-        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, ALT, SWIGLU>), dim3(std::min(mt * nt, 256 * PER_CU)), dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
+static void launch_int8_form(const LinI8Args &a, int tiles, int form, hipStream_t s) {
+#define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST, ALT, PER_CU) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \
+        hipLaunchKernelGGL((linear_int8_tile_kernel<BM, BN, WM, WN, KS, ST, ALT, SWIGLU>), dim3((unsigned)std::min<long>((long)mt * nt, 256 * PER_CU)), \
+                           dim3(WM * WN * 64), 0, s, a, mt, nt); } while (0)
 #define QTTS_SPLIT_I8(TM, TN, NW, U) hipLaunchKernelGGL((linear_int8_split_kernel<TM, TN, NW, U, SWIGLU>), \
         dim3(ceil_div(tiles, TN), ceil_div(a.M, 16 * TM)), dim3(NW * 64), 0, s, a)
     switch (form) {
-    case 1: QTTS_SPLIT_I8(1, 1, 4, 4); break;
-    case 2: QTTS_SPLIT_I8(1, 1, 8, 4); break;
-    case 3: QTTS_SPLIT_I8(1, 2, 8, 4); break;
-    case 4: QTTS_SPLIT_I8(2, 1, 8, 4); break;
-    case 5: QTTS_SPLIT_I8(2, 2, 8, 2); break;
-    case 6: QTTS_SPLIT_I8(2, 2, 8, 4); break;
-    case 7: QTTS_SPLIT_I8(4, 2, 8, 2); break;
-    case 8: QTTS_SPLIT_I8(2, 2, 4, 4); break;
-    case 9: QTTS_SPLIT_I8(4, 2, 4, 2); break;
-    case 10: QTTS_SPLIT_I8(2, 4, 8, 2); break;
-    case 11: QTTS_SPLIT_I8(4, 4, 8, 2); break;
-    case 12: QTTS_SPLIT_I8(4, 4, 4, 2); break;
-    case 13: QTTS_SPLIT_I8(1, 1, 16, 4); break;
-    case 14: QTTS_SPLIT_I8(1, 2, 4, 4); break;
-    case 15: QTTS_SPLIT_I8(1, 1, 16, 2); break;
-    case 16: QTTS_SPLIT_I8(1, 1, 8, 6); break;
-    case 17: QTTS_SPLIT_I8(2, 4, 4, 2); break;
-    case 18: QTTS_SPLIT_I8(4, 4, 8, 1); break;
-    case 21: QTTS_TILE_I8(64, 64, 2, 2, 2, 4, false); break;
-    case 22: QTTS_TILE_I8(64, 64, 2, 2, 2, 8, false); break;
-    case 23: QTTS_TILE_I8(128, 128, 2, 2, 1, 5, false); break;
-    case 24: QTTS_TILE_I8(128, 128, 2, 2, 2, 4, false); break;
-    case 25: QTTS_TILE_I8(128, 128, 2, 2, 2, 3, false); break;
-    case 26: QTTS_TILE_I8(256, 256, 2, 4, 1, 3, false); break;
-    case 27: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, false); break;
-    case 29: QTTS_TILE_I8(256, 256, 4, 2, 1, 3, false); break;
-    case 30: QTTS_TILE_I8(256, 256, 2, 4, 2, 2, false); break;
-    case 31: QTTS_TILE_I8(256, 128, 4, 2, 1, 5, false); break;
-    case 32: QTTS_TILE_I8(128, 256, 2, 4, 1, 3, false); break;
-    case 33: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, false); break;
-    case 40: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, true); break;
-    case 42: QTTS_TILE_I8(256, 256, 4, 2, 1, 3, true); break;
-    case 43: QTTS_TILE_I8(256, 256, 2, 4, 2, 2, true); break;
-    case 44: QTTS_TILE_I8(128, 256, 2, 4, 1, 4, true); break;
-    case 45: QTTS_TILE_I8(256, 128, 4, 2, 1, 4, true); break;
-    case 46: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, true); break;
-    case 47: QTTS_TILE_I8(128, 256, 2, 4, 2, 3, true); break;
-    case 48: QTTS_TILE_I8(128, 128, 2, 4, 2, 4, true); break;
-    case 34: QTTS_TILE_I8(128, 64, 2, 2, 2, 4, false); break;
+    case 0: QTTS_SPLIT_I8(1, 1, 4, 4); break;
+    case 1: QTTS_SPLIT_I8(1, 1, 8, 4); break;
+    case 2: QTTS_SPLIT_I8(1, 2, 4, 4); break;
+    case 3: QTTS_SPLIT_I8(2, 2, 8, 2); break;
+    case 4: QTTS_SPLIT_I8(2, 4, 8, 2); break;
+    case 5: QTTS_TILE_I8(64, 64, 2, 2, 2, 4, false, 2); break;
+    case 6: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, false, 2); break;
+    case 7: QTTS_TILE_I8(128, 128, 2, 4, 2, 4, true, 1); break;
+    case 8: QTTS_TILE_I8(128, 256, 2, 4, 2, 3, true, 1); break;
+    case 9: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, true, 1); break;
     }
 #undef QTTS_TILE_I8
 #undef QTTS_SPLIT_I8
-}
-
-static int launch_linear_int8(const char *who, LinI8Args a, bool swiglu, hipStream_t s) {
-    const int tiles = ceil_div(a.N, swiglu ? 8 : 16);
-    const int form = g_i8_form ? g_i8_form : a.M >= 2048 ? 27 : a.M >= 512 ? 24 : 7;
-    QCHECK(form >= 20 || ceil_div(a.M, 16) <= 65535, "%s: M=%d", who, a.M);
-    if (swiglu) launch_form_int8<true>(a, tiles, form, s);
-    else launch_form_int8<false>(a, tiles, form, s);
-    QLAUNCH();
-    return QTTS_OK;
 }
 
 // The largest of 2, 4, 8, 16 that divides every row's address.
@@ -768,7 +768,7 @@ static int linear_int8_checked(const char *who, const void *x, int ldx, const fl
                                const float *us, const void *bias, const void *res, int ldr, void *out, int ldo, int M, int N,
                                int K, bool swiglu, qtts_stream_t stream) {
     QCHECK(x && xs && wp && ws && out && (!swiglu || us), "%s: null pointer", who);
-    QCHECK(M > 0 && N > 0 && K > 0 && K <= I8_MAX_K && N <= 0x3ffffff0, "%s: bad shape M=%d N=%d K=%d (K <= %d)", who, M, N, K, I8_MAX_K);
+    QCHECK(M > 0 && N > 0 && K > 0 && K <= I8_MAX_K && N <= 0x3ffffff, "%s: bad shape M=%d N=%d K=%d (K <= %d)", who, M, N, K, I8_MAX_K);
     QCHECK(ldx % 16 == 0 && ldx >= K, "%s: x row stride %d too small or not a multiple of 16", who, ldx);
     QCHECK(ldo >= N && (!res || ldr >= N), "%s: row strides ldo=%d ldr=%d < N=%d", who, ldo, ldr, N);
     QCHECK((((uintptr_t)x | (uintptr_t)wp) & 15) == 0 && (((uintptr_t)xs | (uintptr_t)ws | (uintptr_t)us) & 3) == 0 &&
@@ -779,7 +779,11 @@ static int linear_int8_checked(const char *who, const void *x, int ldx, const fl
     a.M = M; a.N = N; a.K = K; a.ksteps = i8_ksteps(K);
     a.ov = row_alignment(out, ldo);
     a.rv = row_alignment(res, ldr);
-    return launch_linear_int8(who, a, swiglu, (hipStream_t)stream);
+    const int tiles = ceil_div(N, swiglu ? 8 : 16), form = choose_int8_form(M, 16 * tiles, K);
+    if (swiglu) launch_int8_form<true>(a, tiles, form, (hipStream_t)stream);
+    else launch_int8_form<false>(a, tiles, form, (hipStream_t)stream);
+    QLAUNCH();
+    return QTTS_OK;
 }
 
 extern "C" int qtts_linear_int8(const void *x, int ldx, const float *x_scales, const void *w_packed, const float *w_scales,
