@@ -56,50 +56,89 @@ __device__ __forceinline__ uint32_t pack4_i8(float a, float b, float c, float d)
     return lo | (hi << 16);
 }
 
-// A row per T = 64 * W threads; thread t holds the 8-column chunks t, t + T, ... (CH of them) as bf16 across both
-// reductions, so x, delta and the weights are read once and nothing is read back.
-template <int W, int CH, bool NORM, bool VEC>
-__global__ __launch_bounds__(W * 64) void rows_int8_kernel(RowsI8Args a) {
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u32(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+    v = max(v, dpp_u32<0xB1>(v));          // as row16_sum
+    v = max(v, dpp_u32<0x4E>(v));
+    v = max(v, dpp_u32<0x141>(v));
+    v = max(v, dpp_u32<0x140>(v));
+    v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+    return max(v, (uint32_t)__shfl_xor((int)v, 32));
+}
+// A row's scale from the bits of its largest magnitude.  NaN and infinity stay: the whole row then stands for NaN.
+__device__ __forceinline__ float i8_scale(uint32_t top) {
+    const float s = __uint_as_float(top) / 127.0f;
+    return s < I8_TINY ? I8_TINY : s;
+}
+// Eight columns from k0 on; inv 0 is a row that is not finite, and stands for zeros.
+__device__ __forceinline__ void store8_i8(int8_t *row, int k0, int K, float (&v)[8], float inv) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = inv != 0.f ? v[j] * inv : 0.f;
+    const uint2 p = make_uint2(pack4_i8(v[0], v[1], v[2], v[3]), pack4_i8(v[4], v[5], v[6], v[7]));
+    if (k0 + 8 <= K) *reinterpret_cast<uint2 *>(row + k0) = p;
+    else
+        for (int j = 0; j < K - k0; ++j) row[k0 + j] = (int8_t)((j < 4 ? p.x >> (8 * j) : p.y >> (8 * (j - 4))) & 0xff);
+}
+
+// A row per T = 64 * W threads, R rows a workgroup; thread t of a row holds the 8-column chunks t, t + T, ... (CH of them) as
+// bf16 across both reductions, so x, delta and the weights are read once and nothing is read back.  All of a thread's
+// requests go out before its first store: sum may be x or delta, and a load behind a store that may alias waits for it.
+template <int W, int R, int CH, bool NORM, bool VEC>
+__global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
     constexpr int T = W * 64;
+    static_assert(W == 1 || R == 1, "one row a workgroup, or one wave a row");
     __shared__ float red_f[W];
     __shared__ uint32_t red_u[W];
-    const int t = threadIdx.x;
-    for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
+    const int t = threadIdx.x % T;
+    for (int m = blockIdx.x * R + threadIdx.x / T; m < a.M; m += gridDim.x * R) {
         const bf16_t *xr = a.x + (size_t)m * a.ldx;
+        const uint4 zero = make_uint4(0, 0, 0, 0);
         Frag h[CH], wv[CH];
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k0 = (c * T + t) * 8;
-            h[c].u = k0 < a.K ? load8<VEC>(xr, k0, a.K) : make_uint4(0, 0, 0, 0);
+            h[c].u = k0 < a.K ? load8<VEC>(xr, k0, a.K) : zero;
         }
-        if (NORM && a.delta) {
-            const bf16_t *dr = a.delta + (size_t)m * a.ldd;
-            bf16_t *sr = a.sum + (size_t)m * a.lds;
+        if (NORM) {
+            Frag d[CH];
+            if (a.delta) {
+                const bf16_t *dr = a.delta + (size_t)m * a.ldd;
+#pragma unroll
+                for (int c = 0; c < CH; ++c) {
+                    const int k0 = (c * T + t) * 8;
+                    d[c].u = k0 < a.K ? load8<VEC>(dr, k0, a.K) : zero;
+                }
+            }
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int k0 = (c * T + t) * 8;
-                if (k0 >= a.K) continue;
-                Frag d;
-                d.u = load8<VEC>(dr, k0, a.K);
+                wv[c].u = k0 < a.K ? load8<VEC>(a.w, k0, a.K) : zero;
+            }
+            if (a.delta) {
+                bf16_t *sr = a.sum + (size_t)m * a.lds;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) h[c].h[j] = f2bf(bf2f(h[c].h[j]) + bf2f(d.h[j]));
-                store8<VEC>(sr, k0, a.K, h[c].u);
+                for (int c = 0; c < CH; ++c) {
+                    const int k0 = (c * T + t) * 8;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h[c].h[j] = f2bf(bf2f(h[c].h[j]) + bf2f(d[c].h[j]));
+                    if (k0 < a.K) store8<VEC>(sr, k0, a.K, h[c].u);
+                }
             }
         }
         float rstd = 1.0f;
         if (NORM) {
-#pragma unroll
-            for (int c = 0; c < CH; ++c) {
-                const int k0 = (c * T + t) * 8;
-                wv[c].u = k0 < a.K ? load8<VEC>(a.w, k0, a.K) : make_uint4(0, 0, 0, 0);
-            }
             float ss = 0.f;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) { const float v = bf2f(h[c].h[j]); ss += v * v; }
             }
-            for (int o = 32; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+            ss = row16_sum(ss);
+            ss += __shfl_xor(ss, 16);
+            ss += __shfl_xor(ss, 32);
             if (W > 1) {
                 if ((t & 63) == 0) red_f[t >> 6] = ss;
                 __syncthreads();
@@ -122,7 +161,7 @@ __global__ __launch_bounds__(W * 64) void rows_int8_kernel(RowsI8Args a) {
                 top = max(top, __float_as_uint(v) & 0x7fffffffu);
             }
         }
-        for (int o = 32; o > 0; o >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o));
+        top = wave_max(top);
         if (W > 1) {
             if ((t & 63) == 0) red_u[t >> 6] = top;
             __syncthreads();
@@ -131,10 +170,10 @@ __global__ __launch_bounds__(W * 64) void rows_int8_kernel(RowsI8Args a) {
             for (int i = 0; i < W; ++i) top = max(top, red_u[i]);
             if (m + gridDim.x < (unsigned)a.M) __syncthreads();      // the next row writes red_* again
         }
-        float s = __uint_as_float(top) / 127.0f;
-        if (s < I8_TINY) s = I8_TINY;                     // NaN and infinity stay: the whole row then stands for NaN
+        const float s = i8_scale(top);
         const float inv = top < 0x7f800000u ? 1.0f / s : 0.f;
         if (t == 0) a.scales[m] = s;
+        if (CH > 2) asm volatile("" : "+v"(rstd));        // the products again, rather than 8 CH of them kept in registers
         int8_t *qr = a.q + (size_t)m * a.ldq;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -145,28 +184,106 @@ __global__ __launch_bounds__(W * 64) void rows_int8_kernel(RowsI8Args a) {
             for (int j = 0; j < 8; ++j) {
                 v[j] = bf2f(h[c].h[j]);
                 if (NORM) v[j] = v[j] * rstd * bf2f(wv[c].h[j]);
-                v[j] = inv != 0.f ? v[j] * inv : 0.f;     // a row that is not finite: zeros
             }
-            const uint2 p = make_uint2(pack4_i8(v[0], v[1], v[2], v[3]), pack4_i8(v[4], v[5], v[6], v[7]));
-            if (k0 + 8 <= a.K) *reinterpret_cast<uint2 *>(qr + k0) = p;
-            else
-                for (int j = 0; j < a.K - k0; ++j) qr[k0 + j] = (int8_t)((j < 4 ? p.x >> (8 * j) : p.y >> (8 * (j - 4))) & 0xff);
+            store8_i8(qr, k0, a.K, v, inv);
         }
     }
 }
 
+// Rows too long for registers: three walks over the row, the second and third of them out of L2 - h is read back from where
+// the first walk wrote it (sum), or from x.  300 rows of 40000 columns: see launch_rows_int8.
+template <bool NORM, bool VEC>
+__global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
+    __shared__ float red_f[16];
+    __shared__ uint32_t red_u[16];
+    const int t = threadIdx.x;
+    for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
+        const bf16_t *xr = a.x + (size_t)m * a.ldx, *hr = xr;
+        float rstd = 1.0f;
+        if (NORM) {
+            float ss = 0.f;
+            const bf16_t *dr = a.delta ? a.delta + (size_t)m * a.ldd : nullptr;
+            bf16_t *sr = a.delta ? a.sum + (size_t)m * a.lds : nullptr;
+#pragma unroll 2
+            for (int k0 = t * 8; k0 < a.K; k0 += 8192) {
+                Frag h, d;
+                h.u = load8<VEC>(xr, k0, a.K);
+                if (dr) {
+                    d.u = load8<VEC>(dr, k0, a.K);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) h.h[j] = f2bf(bf2f(h.h[j]) + bf2f(d.h[j]));
+                    store8<VEC>(sr, k0, a.K, h.u);
+                }
+#pragma unroll
+                for (int j = 0; j < 8; ++j) { const float v = bf2f(h.h[j]); ss += v * v; }
+            }
+            if (dr) hr = sr;
+            ss = row16_sum(ss);
+            ss += __shfl_xor(ss, 16);
+            ss += __shfl_xor(ss, 32);
+            if ((t & 63) == 0) red_f[t >> 6] = ss;
+            __syncthreads();
+            ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) ss += red_f[i];
+            rstd = 1.0f / sqrtf(ss / (float)a.K + a.eps);
+        }
+        auto chunk = [&](int k0, float (&v)[8]) {
+            Frag h, w;
+            h.u = load8<VEC>(hr, k0, a.K);
+            if (NORM) w.u = load8<VEC>(a.w, k0, a.K);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                v[j] = bf2f(h.h[j]);
+                if (NORM) v[j] = k0 + j < a.K ? v[j] * rstd * bf2f(w.h[j]) : 0.f;
+            }
+        };
+        uint32_t top = 0;
+#pragma unroll 4
+        for (int k0 = t * 8; k0 < a.K; k0 += 8192) {
+            float v[8];
+            chunk(k0, v);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+        }
+        top = wave_max(top);
+        if ((t & 63) == 0) red_u[t >> 6] = top;
+        __syncthreads();
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max(top, red_u[i]);
+        if (m + gridDim.x < (unsigned)a.M) __syncthreads();          // the next row writes red_* again
+        const float s = i8_scale(top), inv = top < 0x7f800000u ? 1.0f / s : 0.f;
+        if (t == 0) a.scales[m] = s;
+        int8_t *qr = a.q + (size_t)m * a.ldq;
+#pragma unroll 4
+        for (int k0 = t * 8; k0 < a.K; k0 += 8192) {
+            float v[8];
+            chunk(k0, v);
+            store8_i8(qr, k0, a.K, v, inv);
+        }
+    }
+}
+
+// Threads per row.  Few rows: as many as leave a chunk or two each, the launch is a chain of latencies (8 rows of 6144, with
+// delta: 4.2 us with 512 threads, 4.7 with 256, 5.0 with 64).  Many rows: fewer waves a row and more rows in flight
+// (8192 rows of 6144 with delta: 65 us, 5.4 TB/s, with 256 threads, 72 with 512; 16384 of 2048: 44.5 us with 128, 46.1 with 256,
+// 61 with 512; 16384 of 256: 12 us with a wave, 26 with 256 threads).
 template <bool NORM, bool VEC>
 static void launch_rows_int8(const RowsI8Args &a, hipStream_t s) {
-    const dim3 grid(std::min(a.M, 1 << 20));       // rows beyond that in turns: a launch takes fewer than 2^32 threads
-#define QTTS_ROWS_I8(W, CH) if (a.K <= W * 64 * 8 * CH) { \
-        hipLaunchKernelGGL((rows_int8_kernel<W, CH, NORM, VEC>), grid, dim3(W * 64), 0, s, a); return; }
-    QTTS_ROWS_I8(4, 1)
-    QTTS_ROWS_I8(4, 2)
-    QTTS_ROWS_I8(4, 4)
-    QTTS_ROWS_I8(16, 2)
-    QTTS_ROWS_I8(16, 4)
-    QTTS_ROWS_I8(16, 8)
-    QTTS_ROWS_I8(16, 16)
+#define QTTS_ROWS_I8(W, R, CH, WHEN) if (a.K <= W * 64 * 8 * CH && (WHEN)) { \
+        const dim3 grid(std::min(ceil_div(a.M, R), 1 << 20));       /* rows beyond that in turns: a launch takes fewer than 2^32 threads */ \
+        hipLaunchKernelGGL((rows_int8_kernel<W, R, CH, NORM, VEC>), grid, dim3(W * R * 64), 0, s, a); return; }
+    QTTS_ROWS_I8(1, 4, 1, true)              // up to 512 columns
+    QTTS_ROWS_I8(2, 1, 1, true)              // 1024
+    QTTS_ROWS_I8(2, 1, 2, a.M >= 4096)       // 2048
+    QTTS_ROWS_I8(4, 1, 1, true)
+    QTTS_ROWS_I8(4, 1, 2, a.M >= 2048)       // 4096
+    QTTS_ROWS_I8(8, 1, 1, true)
+    QTTS_ROWS_I8(4, 1, 3, a.M >= 2048)       // 6144
+    QTTS_ROWS_I8(8, 1, 2, true)              // 8192
+    QTTS_ROWS_I8(16, 1, 2, true)             // 16384
+    hipLaunchKernelGGL((rows_int8_long_kernel<NORM, VEC>), dim3(std::min(a.M, 1 << 20)), dim3(1024), 0, s, a);
 #undef QTTS_ROWS_I8
 }
 
