@@ -28,20 +28,25 @@ struct RowsI8Args {
     int M, K;
 };
 
-// 8 columns from k0 on of a row; columns behind the last are zeros.  VEC: rows are 16-byte aligned.
-template <bool VEC>
+// bf16 rows may start anywhere: the hardware takes 16- and 8-byte requests at any address, and these types say so.
+typedef u32x4_t u32x4_any __attribute__((aligned(2)));
+typedef unsigned int u32x2_t __attribute__((ext_vector_type(2)));
+typedef u32x2_t u32x2_any __attribute__((aligned(2)));
+
+// 8 columns from k0 on of a row; columns behind the last are zeros.
 __device__ __forceinline__ uint4 load8(const bf16_t *row, int k0, int K) {
-    if (VEC && k0 + 8 <= K) return *reinterpret_cast<const uint4 *>(row + k0);
     Frag f;
+    if (k0 + 8 <= K) f.n = *reinterpret_cast<const u32x4_any *>(row + k0);
+    else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f.h[j] = k0 + j < K ? row[k0 + j] : (bf16_t)0;
+        for (int j = 0; j < 8; ++j) f.h[j] = k0 + j < K ? row[k0 + j] : (bf16_t)0;
+    }
     return f.u;
 }
-template <bool VEC>
 __device__ __forceinline__ void store8(bf16_t *row, int k0, int K, uint4 v) {
-    if (VEC && k0 + 8 <= K) { *reinterpret_cast<uint4 *>(row + k0) = v; return; }
     Frag f;
     f.u = v;
+    if (k0 + 8 <= K) { *reinterpret_cast<u32x4_any *>(row + k0) = f.n; return; }
 #pragma unroll
     for (int j = 0; j < 8; ++j) if (k0 + j < K) row[k0 + j] = f.h[j];
 }
@@ -86,7 +91,7 @@ __device__ __forceinline__ void store8_i8(int8_t *row, int k0, int K, float (&v)
 // A row per T = 64 * W threads, R rows a workgroup; thread t of a row holds the 8-column chunks t, t + T, ... (CH of them) as
 // bf16 across both reductions, so x, delta and the weights are read once and nothing is read back.  All of a thread's
 // requests go out before its first store: sum may be x or delta, and a load behind a store that may alias waits for it.
-template <int W, int R, int CH, bool NORM, bool VEC>
+template <int W, int R, int CH, bool NORM>
 __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
     constexpr int T = W * 64;
     static_assert(W == 1 || R == 1, "one row a workgroup, or one wave a row");
@@ -100,7 +105,7 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k0 = (c * T + t) * 8;
-            h[c].u = k0 < a.K ? load8<VEC>(xr, k0, a.K) : zero;
+            h[c].u = k0 < a.K ? load8(xr, k0, a.K) : zero;
         }
         if (NORM) {
             Frag d[CH];
@@ -109,13 +114,13 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 #pragma unroll
                 for (int c = 0; c < CH; ++c) {
                     const int k0 = (c * T + t) * 8;
-                    d[c].u = k0 < a.K ? load8<VEC>(dr, k0, a.K) : zero;
+                    d[c].u = k0 < a.K ? load8(dr, k0, a.K) : zero;
                 }
             }
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
                 const int k0 = (c * T + t) * 8;
-                wv[c].u = k0 < a.K ? load8<VEC>(a.w, k0, a.K) : zero;
+                wv[c].u = k0 < a.K ? load8(a.w, k0, a.K) : zero;
             }
             if (a.delta) {
                 bf16_t *sr = a.sum + (size_t)m * a.lds;
@@ -124,7 +129,7 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
                     const int k0 = (c * T + t) * 8;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h[c].h[j] = f2bf(bf2f(h[c].h[j]) + bf2f(d[c].h[j]));
-                    if (k0 < a.K) store8<VEC>(sr, k0, a.K, h[c].u);
+                    if (k0 < a.K) store8(sr, k0, a.K, h[c].u);
                 }
             }
         }
@@ -192,7 +197,7 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 
 // Rows too long for registers: three walks over the row, the second and third of them out of L2 - h is read back from where
 // the first walk wrote it (sum), or from x.  300 rows of 40000 columns: see launch_rows_int8.
-template <bool NORM, bool VEC>
+template <bool NORM>
 __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
     __shared__ float red_f[16];
     __shared__ uint32_t red_u[16];
@@ -207,12 +212,12 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
 #pragma unroll 2
             for (int k0 = t * 8; k0 < a.K; k0 += 8192) {
                 Frag h, d;
-                h.u = load8<VEC>(xr, k0, a.K);
+                h.u = load8(xr, k0, a.K);
                 if (dr) {
-                    d.u = load8<VEC>(dr, k0, a.K);
+                    d.u = load8(dr, k0, a.K);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) h.h[j] = f2bf(bf2f(h.h[j]) + bf2f(d.h[j]));
-                    store8<VEC>(sr, k0, a.K, h.u);
+                    store8(sr, k0, a.K, h.u);
                 }
 #pragma unroll
                 for (int j = 0; j < 8; ++j) { const float v = bf2f(h.h[j]); ss += v * v; }
@@ -230,8 +235,8 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
         }
         auto chunk = [&](int k0, float (&v)[8]) {
             Frag h, w;
-            h.u = load8<VEC>(hr, k0, a.K);
-            if (NORM) w.u = load8<VEC>(a.w, k0, a.K);
+            h.u = load8(hr, k0, a.K);
+            if (NORM) w.u = load8(a.w, k0, a.K);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] = bf2f(h.h[j]);
@@ -269,11 +274,11 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
 // delta: 4.2 us with 512 threads, 4.7 with 256, 5.0 with 64).  Many rows: fewer waves a row and more rows in flight
 // (8192 rows of 6144 with delta: 65 us, 5.4 TB/s, with 256 threads, 72 with 512; 16384 of 2048: 44.5 us with 128, 46.1 with 256,
 // 61 with 512; 16384 of 256: 12 us with a wave, 26 with 256 threads).
-template <bool NORM, bool VEC>
+template <bool NORM>
 static void launch_rows_int8(const RowsI8Args &a, hipStream_t s) {
 #define QTTS_ROWS_I8(W, R, CH, WHEN) if (a.K <= W * 64 * 8 * CH && (WHEN)) { \
         const dim3 grid(std::min(ceil_div(a.M, R), 1 << 20));       /* rows beyond that in turns: a launch takes fewer than 2^32 threads */ \
-        hipLaunchKernelGGL((rows_int8_kernel<W, R, CH, NORM, VEC>), grid, dim3(W * R * 64), 0, s, a); return; }
+        hipLaunchKernelGGL((rows_int8_kernel<W, R, CH, NORM>), grid, dim3(W * R * 64), 0, s, a); return; }
     QTTS_ROWS_I8(1, 4, 1, true)              // up to 512 columns
     QTTS_ROWS_I8(2, 1, 1, true)              // 1024
     QTTS_ROWS_I8(2, 1, 2, a.M >= 4096)       // 2048
@@ -283,7 +288,7 @@ static void launch_rows_int8(const RowsI8Args &a, hipStream_t s) {
     QTTS_ROWS_I8(4, 1, 3, a.M >= 2048)       // 6144
     QTTS_ROWS_I8(8, 1, 2, true)              // 8192
     QTTS_ROWS_I8(16, 1, 2, true)             // 16384
-    hipLaunchKernelGGL((rows_int8_long_kernel<NORM, VEC>), dim3(std::min(a.M, 1 << 20)), dim3(1024), 0, s, a);
+    hipLaunchKernelGGL((rows_int8_long_kernel<NORM>), dim3(std::min(a.M, 1 << 20)), dim3(1024), 0, s, a);
 #undef QTTS_ROWS_I8
 }
 
@@ -294,8 +299,7 @@ extern "C" int qtts_quantize_int8(const void *x, int ldx, void *q, int ldq, floa
     QCHECK(((uintptr_t)x & 1) == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)scales & 3) == 0, "quantize_int8: misaligned pointer");
     RowsI8Args a{};
     a.x = (const bf16_t *)x; a.ldx = ldx; a.q = (int8_t *)q; a.ldq = ldq; a.scales = scales; a.M = M; a.K = K;
-    if (((uintptr_t)x & 15) == 0 && ldx % 8 == 0) launch_rows_int8<false, true>(a, (hipStream_t)stream);
-    else launch_rows_int8<false, false>(a, (hipStream_t)stream);
+    launch_rows_int8<false>(a, (hipStream_t)stream);
     QLAUNCH();
     return QTTS_OK;
 }
@@ -312,10 +316,7 @@ extern "C" int qtts_rmsnorm_int8(const void *x, int ldx, const void *delta, int 
     RowsI8Args a{};
     a.x = (const bf16_t *)x; a.ldx = ldx; a.delta = (const bf16_t *)delta; a.ldd = ldd; a.w = (const bf16_t *)w; a.eps = eps;
     a.sum = (bf16_t *)sum; a.lds = lds; a.q = (int8_t *)q; a.ldq = ldq; a.scales = scales; a.M = M; a.K = H;
-    const bool vec = (((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)sum) & 15) == 0 && ldx % 8 == 0 &&
-                     (!delta || (ldd % 8 == 0 && lds % 8 == 0));
-    if (vec) launch_rows_int8<true, true>(a, (hipStream_t)stream);
-    else launch_rows_int8<true, false>(a, (hipStream_t)stream);
+    launch_rows_int8<true>(a, (hipStream_t)stream);
     QLAUNCH();
     return QTTS_OK;
 }
@@ -379,7 +380,6 @@ struct LinI8Args {
     const bf16_t *bias, *res; int ldr;
     bf16_t *out; int ldo;
     int M, N, K, ksteps;           // N: output columns; ksteps: of a packed tile
-    int ov, rv;                    // output / residual rows: bytes they are aligned to
 };
 
 // What follows a sum, in the same operations in every kernel: a row's result does not depend on the form it came from.
@@ -402,9 +402,7 @@ __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int til
             const int nn = min(n + j, a.N - 1);
             y[j] = i8_swiglu(acc[j], acc[2 + j], xs, a.ws[nn], a.us[nn]);
         }
-        if (a.ov >= 4 && n + 2 <= a.N) *reinterpret_cast<uint32_t *>(o + n) = pack2(y[0], y[1]);
-        else
-            for (int j = 0; j < 2; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
+        for (int j = 0; j < 2; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
         return;
     }
     const int n = 16 * tile + 4 * (lane >> 4);
@@ -417,15 +415,15 @@ __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int til
     }
     if (a.res) {
         const bf16_t *rr = a.res + (size_t)m * a.ldr;
-        if (a.rv >= 8 && full) {
-            const uint2 r = *reinterpret_cast<const uint2 *>(rr + n);
+        if (full) {
+            const u32x2_t r = *reinterpret_cast<const u32x2_any *>(rr + n);
             float p, q;
-            unpack2(r.x, p, q); y[0] += p; y[1] += q;
-            unpack2(r.y, p, q); y[2] += p; y[3] += q;
+            unpack2(r[0], p, q); y[0] += p; y[1] += q;
+            unpack2(r[1], p, q); y[2] += p; y[3] += q;
         } else
             for (int j = 0; j < 4; ++j) y[j] += bf2f(rr[min(n + j, a.N - 1)]);
     }
-    if (a.ov >= 8 && full) *reinterpret_cast<uint2 *>(o + n) = make_uint2(pack2(y[0], y[1]), pack2(y[2], y[3]));
+    if (full) *reinterpret_cast<u32x2_any *>(o + n) = u32x2_t{pack2v(float2_t{y[0], y[1]}), pack2v(float2_t{y[2], y[3]})};
     else
         for (int j = 0; j < 4; ++j) if (n + j < a.N) o[n + j] = f2bf(y[j]);
 }
@@ -701,13 +699,14 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
         }
 #pragma unroll
         for (int j = 0; j < XW; ++j) now.xs[j] = a.xs[min(row0 + 64 * j + lane, a.M - 1)];
-        const bool wide = a.N % OUT == 0 && a.ov >= 2 * OUT && (SWIGLU || !a.res || a.rv == 16);      // whole pieces, aligned
+        const int whole = a.N / OUT * OUT;                         // the columns behind these are stored one by one
+        const bool rest = whole < a.N && whole >= nw && whole < nw + TN * (SWIGLU ? 8 : 16);      // they are this wave's
         // Residual rows are requested RB passes ahead.  Behind the last row the last is read: the loads stay unconditional.
         constexpr int PASSES = TM / HT * NP, RB = SWIGLU ? 1 : PASSES < 8 ? PASSES : 8;
         u32x4_t rf[RB];
-        const bool add = !SWIGLU && wide && a.res;
+        const bool add = !SWIGLU && a.res && whole > 0;
         auto residual = [&](int pass) {
-            return *reinterpret_cast<const u32x4_t *>(a.res + (size_t)min(row0 + lane / LPR + pass * RPP, a.M - 1) * a.ldr + min(n0, a.N - OUT));
+            return (u32x4_t)*reinterpret_cast<const u32x4_any *>(a.res + (size_t)min(row0 + lane / LPR + pass * RPP, a.M - 1) * a.ldr + min(n0, whole - OUT));
         };
         if (add) {
 #pragma unroll
@@ -745,11 +744,11 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
             }
         };
         auto row_scale = [&](int row) { return __shfl(now.xs[row >> 6], (row & 63) + lrow); };    // row: a constant, a multiple of RPP
-        const int have = n0 < a.N ? a.M - row0 - lrow : 0;      // rows from this lane's first on
+        const int have = n0 < whole ? a.M - row0 - lrow : 0;      // rows from this lane's first on
         bf16_t *op = a.out + (size_t)(row0 + lrow) * a.ldo + n0;
         const size_t ostep = (size_t)RPP * a.ldo;
-        // every pass stores something: the rows are there, and the wave's first column
-        loose = wide && row0 + TM * 16 <= a.M && nw < a.N ? ST - 1 : 0;
+        // every pass stores something: the rows are there, and the wave's first columns
+        loose = row0 + TM * 16 <= a.M && nw < whole ? ST - 1 : 0;
 #pragma unroll
         for (int h = 0; h < TM; h += HT) {
 #pragma unroll
@@ -757,47 +756,47 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 #pragma unroll
                 for (int j = 0; j < TN; ++j) mine[(16 * i + r) * (TN * 4) + ((4 * j + g) ^ (r & CMASK))] = acc[h + i][j];
             __builtin_amdgcn_wave_barrier();
-            if (wide) {
 #pragma unroll
-                for (int p = 0; p < NP; ++p) {
-                    float y[OUT];
-                    outputs(p, row_scale(h * 16 + p * RPP), y);
-                    if (add) {
-                        const int pass = h / HT * NP + p;
+            for (int p = 0; p < NP; ++p) {
+                float y[OUT];
+                outputs(p, row_scale(h * 16 + p * RPP), y);
+                if (add) {
+                    const int pass = h / HT * NP + p;
 #pragma unroll
-                        for (int j = 0; j < OUT; j += 2) {
-                            float lo, hi;
-                            unpack2(rf[pass % RB][j / 2], lo, hi);
-                            y[j] += lo;
-                            y[j + 1] += hi;
-                        }
-                        if (pass + RB < PASSES) rf[pass % RB] = residual(pass + RB);
+                    for (int j = 0; j < OUT; j += 2) {
+                        float lo, hi;
+                        unpack2(rf[pass % RB][j / 2], lo, hi);
+                        y[j] += lo;
+                        y[j + 1] += hi;
                     }
-                    uint32_t packed[OUT / 2];
-#pragma unroll
-                    for (int j = 0; j < OUT; j += 2) packed[j / 2] = pack2v(float2_t{y[j], y[j + 1]});
-                    if (h * 16 + p * RPP < have) {
-                        if constexpr (OUT == 8) *reinterpret_cast<uint4 *>(op) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
-                        else *reinterpret_cast<uint2 *>(op) = make_uint2(packed[0], packed[1]);
-                    }
-                    op += ostep;
+                    if (pass + RB < PASSES) rf[pass % RB] = residual(pass + RB);
                 }
-            } else {
-                // the last columns, or rows that are not aligned: an output at a time, neighbouring lanes neighbouring columns
-                constexpr int COLS = TN * (SWIGLU ? 8 : 16);
+                uint32_t packed[OUT / 2];
+#pragma unroll
+                for (int j = 0; j < OUT; j += 2) packed[j / 2] = pack2v(float2_t{y[j], y[j + 1]});
+                if (h * 16 + p * RPP < have) {
+                    if constexpr (OUT == 8) *reinterpret_cast<u32x4_any *>(op) = u32x4_t{packed[0], packed[1], packed[2], packed[3]};
+                    else *reinterpret_cast<u32x2_any *>(op) = u32x2_t{packed[0], packed[1]};
+                }
+                op += ostep;
+            }
+            if (rest) {                                            // neighbouring lanes neighbouring columns, 64 / OUT rows at a time
+                const int tc = lane % OUT, n = min(whole + tc, a.N - 1), col = n - nw;
+                const int pc = SWIGLU ? (col >> 1) * 4 + (col & 1) : col;                  // packed column of the sum (of the gate's)
                 const int *flat = reinterpret_cast<const int *>(mine);
-#pragma unroll 4
-                for (int e = lane; e < 16 * HT * COLS; e += 64) {
-                    const int row = e / COLS, col = e % COLS, m = min(row0 + h * 16 + row, a.M - 1), n = min(nw + col, a.N - 1);
-                    const int pc = SWIGLU ? (col >> 1) * 4 + (col & 1) : col;          // packed column of the sum (of the gate's)
+                const float s0 = a.ws[n], s1 = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
+#pragma unroll
+                for (int e = 0; e < 16 * HT * OUT / 64; ++e) {
+                    const int row = e * (64 / OUT) + lane / OUT, m = min(row0 + h * 16 + row, a.M - 1);
                     const int at = (row * (TN * 4) + ((pc >> 2) ^ (row & CMASK))) * 4 + (pc & 3);
+                    const float xs = __shfl(now.xs[h >> 2], (h & 3) * 16 + row);
                     float y;
-                    if (SWIGLU) y = i8_swiglu(flat[at], flat[at + 2], a.xs[m], a.ws[n], a.us[n]);
+                    if (SWIGLU) y = i8_swiglu(flat[at], flat[at + 2], xs, s0, s1);
                     else {
-                        y = i8_scaled(flat[at], a.xs[m], a.ws[n], a.bias ? bf2f(a.bias[n]) : 0.f);
+                        y = i8_scaled(flat[at], xs, s0, s1);
                         if (a.res) y += bf2f(a.res[(size_t)m * a.ldr + n]);
                     }
-                    if (row0 + h * 16 + row < a.M && nw + col < a.N) a.out[(size_t)m * a.ldo + n] = f2bf(y);
+                    if (row0 + h * 16 + row < a.M && whole + tc < a.N) a.out[(size_t)m * a.ldo + n] = f2bf(y);
                 }
             }
             __builtin_amdgcn_wave_barrier();
@@ -875,12 +874,6 @@ static void launch_int8_form(const LinI8Args &a, int tiles, int form, hipStream_
 #undef QTTS_SPLIT_I8
 }
 
-// The largest of 2, 4, 8, 16 that divides every row's address.
-static int row_alignment(const void *p, int ld) {
-    const uintptr_t bits = (uintptr_t)p | ((uintptr_t)ld * 2) | 16;
-    return (int)(bits & (~bits + 1));
-}
-
 static int linear_int8_checked(const char *who, const void *x, int ldx, const float *xs, const void *wp, const float *ws,
                                const float *us, const void *bias, const void *res, int ldr, void *out, int ldo, int M, int N,
                                int K, bool swiglu, qtts_stream_t stream) {
@@ -894,8 +887,6 @@ static int linear_int8_checked(const char *who, const void *x, int ldx, const fl
     a.x = (const int8_t *)x; a.ldx = ldx; a.xs = xs; a.wp = (const uint4 *)wp; a.ws = ws; a.us = us;
     a.bias = (const bf16_t *)bias; a.res = (const bf16_t *)res; a.ldr = ldr; a.out = (bf16_t *)out; a.ldo = ldo;
     a.M = M; a.N = N; a.K = K; a.ksteps = i8_ksteps(K);
-    a.ov = row_alignment(out, ldo);
-    a.rv = row_alignment(res, ldr);
     const int tiles = ceil_div(N, swiglu ? 8 : 16), form = choose_int8_form(M, 16 * tiles, K);
     if (swiglu) launch_int8_form<true>(a, tiles, form, (hipStream_t)stream);
     else launch_int8_form<false>(a, tiles, form, (hipStream_t)stream);
