@@ -2,6 +2,22 @@
 // on MFMA), the fused decode launch, the burst's 2-position prompts.  C ABI in include/qtts_hip.h.
 #include "qtts_common.h"
 
+// Where a product is followed by an addition or subtraction the compiler may fuse the two or not, and decides by what else
+// it does with them: the last bit of a result then changes with the build.  The softmax arithmetic therefore says which it
+// is - __builtin_fmaf where the two are one operation, the functions below where they are two.
+__device__ __forceinline__ float scaled(float score, float scale) {
+#pragma clang fp contract(off)
+    return score * scale;
+}
+__device__ __forceinline__ float below(float score, float maximum) {
+#pragma clang fp contract(off)
+    return score - maximum;
+}
+__device__ __forceinline__ float plus_product(float sum, float a, float b) {
+#pragma clang fp contract(off)
+    return sum + a * b;
+}
+
 // ------------------------------------------------------------------ q/k norm + RoPE + KV store
 // One wave per (token, head); lane i owns dims i and i+64 (the rotate_half pair).
 __global__ __launch_bounds__(64) void qknorm_rope_store_kernel(
@@ -154,14 +170,15 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += qf[h][j] * kf[j];
-            s = row16_sum(s) * scale;
+            const float dot = row16_sum(s);
+            s = scaled(dot, scale);
             if (valid) {
                 const float mn = fmaxf(mx[h], s);
-                const float corr = __expf(mx[h] - mn);
-                const float p = __expf(s - mn);
-                ls[h] = ls[h] * corr + p;
+                const float corr = __expf(below(mx[h], mn));
+                const float p = __expf(__builtin_fmaf(dot, scale, -mn));
+                ls[h] = __builtin_fmaf(ls[h], corr, p);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) acc[h][j] = acc[h][j] * corr + p * vf[j];
+                for (int j = 0; j < 8; ++j) acc[h][j] = __builtin_fmaf(acc[h][j], corr, scaled(p, vf[j]));
                 mx[h] = mn;
             }
         }
@@ -185,8 +202,8 @@ __global__ __launch_bounds__(256) void paged_attn_kernel(
 #pragma unroll
         for (int gI = 0; gI < 16; ++gI) {
             const float wgt = __expf(sm_m[gI][h] - M);      // exp(-inf) = 0 for empty groups
-            L += sm_l[gI][h] * wgt;
-            o += sm_acc[gI][h][d] * wgt;
+            L = __builtin_fmaf(sm_l[gI][h], wgt, L);
+            o = __builtin_fmaf(sm_acc[gI][h][d], wgt, o);
         }
         const int hq = kvh * G + h;
         if (nsplit == 1) {
@@ -220,8 +237,8 @@ __global__ __launch_bounds__(128) void attn_combine_kernel(const float *__restri
     float L = 0.f, o = 0.f;
     for (int s = 0; s < ns; ++s) {
         const float wgt = __expf(part_ml[(p0 + s) * 2] - M);
-        L += part_ml[(p0 + s) * 2 + 1] * wgt;
-        o += part_o[(p0 + s) * 128 + d] * wgt;
+        L = __builtin_fmaf(part_ml[(p0 + s) * 2 + 1], wgt, L);
+        o = __builtin_fmaf(part_o[(p0 + s) * 128 + d], wgt, o);
     }
     out[act_index(row, hq * 128 + d, ldo, opks)] = f2bf(o / L);
 }
@@ -341,14 +358,14 @@ __global__ __launch_bounds__(512) void prefill_attn_mfma_kernel(
             float rmax = NEG;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                sv[i] = (t0 + 4 * g + i) < climit ? sa[i] * scale : NEG;
-                sv[4 + i] = (t0 + 16 + 4 * g + i) < climit ? sb[i] * scale : NEG;
+                sv[i] = (t0 + 4 * g + i) < climit ? scaled(sa[i], scale) : NEG;
+                sv[4 + i] = (t0 + 16 + 4 * g + i) < climit ? scaled(sb[i], scale) : NEG;
                 rmax = fmaxf(rmax, fmaxf(sv[i], sv[4 + i]));
             }
             rmax = fmaxf(rmax, __shfl_xor(rmax, 16));
             rmax = fmaxf(rmax, __shfl_xor(rmax, 32));
             const float mnew = fmaxf(mrun, rmax);
-            const float alpha = __expf(mrun - mnew);                       // 1 while the row has seen nothing
+            const float alpha = __expf(below(mrun, mnew));                       // 1 while the row has seen nothing
             mrun = mnew;
             // a probability enters the second product as the sum of two bf16 numbers (16 mantissa bits), so that the
             // result stays as close to the fp32 softmax of the definition as the per-row kernel's
@@ -356,12 +373,12 @@ __global__ __launch_bounds__(512) void prefill_attn_mfma_kernel(
             Frag pf, pl;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float pr = sv[i] > 0.5f * NEG ? __expf(sv[i] - mnew) : 0.f;
+                const float pr = sv[i] > 0.5f * NEG ? __expf(below(sv[i], mnew)) : 0.f;
                 pf.h[i] = f2bf(pr);
                 pl.h[i] = f2bf(pr - bf2f(pf.h[i]));
                 psum += pr;
             }
-            lrun = lrun * alpha + psum;
+            lrun = __builtin_fmaf(lrun, alpha, psum);
 #pragma unroll
             for (int dt = 0; dt < 8; ++dt) {
                 o[dt] *= alpha;
@@ -405,7 +422,7 @@ __global__ __launch_bounds__(512) void prefill_attn_mfma_kernel(
     for (int k = 0; k < NTG; ++k) {
         const float *pml = reinterpret_cast<const float *>(pa_smem + (size_t)(k * G + h) * PA_WAVE_LDS + 8192);
         wk[k] = __expf(pml[2 * r] - M);
-        L += pml[2 * r + 1] * wk[k];
+        L = plus_product(L, pml[2 * r + 1], wk[k]);
     }
     const float inv = L > 0.f ? 1.0f / L : 0.f;                            // a row without context gives zeros
 #pragma unroll
@@ -414,7 +431,9 @@ __global__ __launch_bounds__(512) void prefill_attn_mfma_kernel(
 #pragma unroll
         for (int k = 0; k < NTG; ++k) {
             const float4_t *po = reinterpret_cast<const float4_t *>(pa_smem + (size_t)(k * G + h) * PA_WAVE_LDS);
-            acc += po[dt * 64 + lane] * wk[k];
+            const float4_t part = po[dt * 64 + lane];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[e] = __builtin_fmaf(part[e], wk[k], acc[e]);
         }
         if (rvalid)
             *reinterpret_cast<uint2 *>(out + act_index(m, hq * 128 + 16 * dt + 4 * g, ldo, opks)) =
@@ -721,7 +740,7 @@ __global__ __launch_bounds__(NG * 16) void attn_decode_fused_kernel(const int32_
             float s = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) s += qf[h][j] * bf2f(kk[i].h[j]);
-            s = row16_sum(s) * p.scale;
+            s = scaled(row16_sum(s), p.scale);
             sc[i][h] = t < ctx ? s : -INFINITY;
         }
     }
@@ -745,10 +764,10 @@ __global__ __launch_bounds__(NG * 16) void attn_decode_fused_kernel(const int32_
 #pragma unroll
         for (int h = 0; h < G; ++h) {
             // a masked score is -inf: its weight is 0 unless the whole group is empty (-inf - -inf), hence the test
-            const float pr = sc[i][h] == -INFINITY ? 0.f : __expf(sc[i][h] - mx[h]);
+            const float pr = sc[i][h] == -INFINITY ? 0.f : __expf(below(sc[i][h], mx[h]));
             ls[h] += pr;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) acc[h][j] += pr * vf[j];
+            for (int j = 0; j < 8; ++j) acc[h][j] = __builtin_fmaf(pr, vf[j], acc[h][j]);
         }
     }
 #pragma unroll
@@ -786,8 +805,8 @@ __global__ __launch_bounds__(NG * 16) void attn_decode_fused_kernel(const int32_
 #pragma unroll
             for (int j = 0; j < MB; ++j) {
                 const float wgt = __expf(mv[g0 + j] - M);  // an empty group: exp(-inf) = 0
-                L += lv[j] * wgt;
-                o += av[j] * wgt;
+                L = __builtin_fmaf(lv[j], wgt, L);
+                o = __builtin_fmaf(av[j], wgt, o);
             }
         }
         const int hq = kvh * G + h;
@@ -847,15 +866,15 @@ __global__ __launch_bounds__(NG * 16) void attn_decode_fused_kernel(const int32_
 #pragma unroll
             for (int s = 0; s < MERGE_MAX; ++s) {
                 const float wgt = __expf(pm[s] - M);
-                L = s < nact ? L + pl[s] * wgt : L;
-                o = s < nact ? o + po[s] * wgt : o;
+                L = s < nact ? plus_product(L, pl[s], wgt) : L;
+                o = s < nact ? plus_product(o, po[s], wgt) : o;
             }
         } else {
             for (int s = 0; s < nact; ++s) M = fmaxf(M, ld_agent(p.part_ml + (p0 + s) * 2));
             for (int s = 0; s < nact; ++s) {
                 const float wgt = __expf(ld_agent(p.part_ml + (p0 + s) * 2) - M);
-                L += ld_agent(p.part_ml + (p0 + s) * 2 + 1) * wgt;
-                o += ld_agent(p.part_o + (p0 + s) * 128 + d) * wgt;
+                L = __builtin_fmaf(ld_agent(p.part_ml + (p0 + s) * 2 + 1), wgt, L);
+                o = __builtin_fmaf(ld_agent(p.part_o + (p0 + s) * 128 + d), wgt, o);
             }
         }
         p.out[act_index(row, hq * 128 + d, p.ldo, p.opks)] = f2bf(o / L);
@@ -1035,16 +1054,15 @@ __global__ __launch_bounds__(64) void attn_pair_kernel(const bf16_t *__restrict_
         s0 += q1[j] * bf2f(kb[0].h[j]);
         s1 += q1[j] * bf2f(kb[1].h[j]);
     }
-    s0 = row16_sum(s0) * scale;
-    s1 = row16_sum(s1) * scale;
-    const float mx = fmaxf(s0, s1);
-    const float p0 = __expf(s0 - mx), p1 = __expf(s1 - mx);
+    s0 = row16_sum(s0);
+    s1 = row16_sum(s1);
+    const float mx = fmaxf(scaled(s0, scale), scaled(s1, scale));
+    const float p0 = __expf(__builtin_fmaf(s0, scale, -mx)), p1 = __expf(__builtin_fmaf(s1, scale, -mx));
     const float L = p0 + p1;
     Frag o;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        float acc = p0 * bf2f(vb[0].h[j]);
-        acc += p1 * bf2f(vb[1].h[j]);
+        const float acc = __builtin_fmaf(p0, bf2f(vb[0].h[j]), scaled(p1, bf2f(vb[1].h[j])));
         o.h[j] = f2bf(acc / L);
     }
     *reinterpret_cast<uint4 *>(out + act_index(2 * seq + 1, hq * 128 + 8 * l16, ldo, opks)) = o.u;
