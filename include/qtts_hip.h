@@ -105,8 +105,9 @@ int qtts_linear_swiglu_fp8(const void *x, int ldx, const void *w_gate_up_fp8_pac
  * fp32 scale each, a row standing for q * scale.  A product's integer sum is exact (int32, K <= 131071); what follows it is
  * fp32 with ONE rounding, to bf16, at the store.  int8 activations are [M, ld] with ld % 16 == 0, 16-byte aligned: the bytes
  * K .. round_up(K, 16) of every row (the last one included) must be readable, whatever they hold, and are never written.
- * M, N, I >= 1 and K, H >= 1 are free of multiples, bf16 rows of strides and alignment.  A row that holds a NaN or an infinity gets a scale that is NaN or infinite and
- * q = 0: everything computed from that row is NaN, no other row is touched.
+ * M, N, I >= 1 and K, H >= 1 are free of multiples, bf16 rows of strides and alignment; a row's result does not depend on
+ * the number of rows, nor on the rows beside it.  M <= 2139095040, N and I <= 67108863.  A row that holds a NaN or an
+ * infinity gets a scale that is NaN or infinite and q = 0: everything computed from that row is NaN, no other row is touched.
  *
  * qtts_quantize_int8: scales[m] = max(max|x[m]| / 127, 2^-126), q[m] = rint(x[m] / scales[m]), |q| <= 127.
  * (Also quantises F.linear weights [N,K] per output channel, for qtts_pack_weight_int8.)

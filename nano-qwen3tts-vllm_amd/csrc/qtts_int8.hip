@@ -13,9 +13,11 @@
 typedef int int4_t __attribute__((ext_vector_type(4)));
 
 static constexpr int I8_MAX_K = 131071;            // int32 holds the sum of this many products of two int8 values
+static constexpr int I8_MAX_ROWS = 0x7f800000;     // row numbers a launch's rounding up passes still fit an int
+static constexpr int I8_MAX_N = 0x3ffffff;
 static constexpr float I8_TINY = 0x1p-126f;        // smallest scale: its reciprocal is finite, rows of zeros stay zeros
 
-__host__ __device__ static inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+__host__ __device__ static inline int ceil_div(int a, int b) { return (a - 1) / b + 1; }       // a, b > 0
 
 // ------------------------------------------------------------------ rows -> int8
 struct RowsI8Args {
@@ -95,7 +97,7 @@ template <int W, int R, int CH, bool NORM>
 __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
     constexpr int T = W * 64;
     static_assert(W == 1 || R == 1, "one row a workgroup, or one wave a row");
-    __shared__ float red_f[W];
+    __shared__ float red_f[W * CH];
     __shared__ uint32_t red_u[W];
     const int t = threadIdx.x % T;
     for (int m = blockIdx.x * R + threadIdx.x / T; m < a.M; m += gridDim.x * R) {
@@ -135,21 +137,29 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
         }
         float rstd = 1.0f;
         if (NORM) {
-            float ss = 0.f;
+            // Squares are added up per 512 columns (a chunk's 8, then the 64 lanes of a wave), then in the order of the columns:
+            // the same sum, and the same row, whatever number of threads the launch chose.
+            float part[CH], ss = 0.f;
 #pragma unroll
             for (int c = 0; c < CH; ++c) {
+                part[c] = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) { const float v = bf2f(h[c].h[j]); ss += v * v; }
+                for (int j = 0; j < 8; ++j) { const float v = bf2f(h[c].h[j]); part[c] = __builtin_fmaf(v, v, part[c]); }
+                part[c] = row16_sum(part[c]);
+                part[c] += __shfl_xor(part[c], 16);
+                part[c] += __shfl_xor(part[c], 32);
             }
-            ss = row16_sum(ss);
-            ss += __shfl_xor(ss, 16);
-            ss += __shfl_xor(ss, 32);
             if (W > 1) {
-                if ((t & 63) == 0) red_f[t >> 6] = ss;
-                __syncthreads();
-                ss = 0.f;
+                if ((t & 63) == 0) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) ss += red_f[i];
+                    for (int c = 0; c < CH; ++c) red_f[c * W + (t >> 6)] = part[c];
+                }
+                __syncthreads();
+#pragma unroll
+                for (int i = 0; i < W * CH; ++i) ss += red_f[i];
+            } else {
+#pragma unroll
+                for (int c = 0; c < CH; ++c) ss += part[c];
             }
             rstd = 1.0f / sqrtf(ss / (float)a.K + a.eps);
         }
@@ -294,7 +304,7 @@ static void launch_rows_int8(const RowsI8Args &a, hipStream_t s) {
 
 extern "C" int qtts_quantize_int8(const void *x, int ldx, void *q, int ldq, float *scales, int M, int K, qtts_stream_t stream) {
     QCHECK(x && q && scales, "quantize_int8: null pointer");
-    QCHECK(M > 0 && K > 0 && K <= I8_MAX_K, "quantize_int8: bad shape M=%d K=%d (K <= %d)", M, K, I8_MAX_K);
+    QCHECK(M > 0 && M <= I8_MAX_ROWS && K > 0 && K <= I8_MAX_K, "quantize_int8: bad shape M=%d K=%d (M <= %d, K <= %d)", M, K, I8_MAX_ROWS, I8_MAX_K);
     QCHECK(ldx >= K && ldq >= K && ldq % 16 == 0, "quantize_int8: row strides ldx=%d ldq=%d (need ldx >= K, ldq >= K, ldq %% 16 == 0)", ldx, ldq);
     QCHECK(((uintptr_t)x & 1) == 0 && ((uintptr_t)q & 15) == 0 && ((uintptr_t)scales & 3) == 0, "quantize_int8: misaligned pointer");
     RowsI8Args a{};
@@ -308,9 +318,10 @@ extern "C" int qtts_rmsnorm_int8(const void *x, int ldx, const void *delta, int 
                                  void *q, int ldq, float *scales, int M, int H, qtts_stream_t stream) {
     QCHECK(x && w && q && scales, "rmsnorm_int8: null pointer");
     QCHECK(!delta == !sum, "rmsnorm_int8: delta and sum come together");
-    QCHECK(M > 0 && H > 0 && H <= I8_MAX_K, "rmsnorm_int8: bad shape M=%d H=%d (H <= %d)", M, H, I8_MAX_K);
+    QCHECK(M > 0 && M <= I8_MAX_ROWS && H > 0 && H <= I8_MAX_K, "rmsnorm_int8: bad shape M=%d H=%d (M <= %d, H <= %d)", M, H, I8_MAX_ROWS, I8_MAX_K);
     QCHECK(ldx >= H && ldq >= H && ldq % 16 == 0 && (!delta || (ldd >= H && lds >= H)),
            "rmsnorm_int8: row strides ldx=%d ldd=%d lds=%d ldq=%d (need >= H, ldq %% 16 == 0)", ldx, ldd, lds, ldq);
+    QCHECK((sum != x || lds == ldx) && (!sum || sum != delta || lds == ldd), "rmsnorm_int8: sum in the place of x or delta needs its row stride");
     QCHECK((((uintptr_t)x | (uintptr_t)delta | (uintptr_t)w | (uintptr_t)sum) & 1) == 0 && ((uintptr_t)q & 15) == 0 &&
            ((uintptr_t)scales & 3) == 0, "rmsnorm_int8: misaligned pointer");
     RowsI8Args a{};
@@ -345,18 +356,18 @@ __global__ __launch_bounds__(256) void pack_int8_kernel(const int8_t *__restrict
 }
 
 extern "C" size_t qtts_packed_weight_int8_bytes(int N, int K) {
-    if (N <= 0 || K <= 0 || N > 0x7ffffff0 || K > I8_MAX_K) return 0;
+    if (N <= 0 || K <= 0 || N > I8_MAX_N || K > I8_MAX_K) return 0;
     return (size_t)ceil_div(N, 16) * i8_ksteps(K) * 1024;
 }
 extern "C" size_t qtts_packed_gate_up_int8_bytes(int I, int K) {
-    if (I <= 0 || K <= 0 || I > 0x3ffffff0 || K > I8_MAX_K) return 0;
+    if (I <= 0 || K <= 0 || I > I8_MAX_N || K > I8_MAX_K) return 0;
     return (size_t)ceil_div(I, 8) * i8_ksteps(K) * 1024;
 }
 
-static int pack_int8(const char *who, const void *w, const void *up, int ldw, void *packed, int N, int K, int tiles, hipStream_t s) {
-    QCHECK(N > 0 && K > 0 && K <= I8_MAX_K && ldw >= K, "%s: bad shape N=%d K=%d ldw=%d (K <= %d)", who, N, K, ldw, I8_MAX_K);
+static int pack_int8(const char *who, const void *w, const void *up, int ldw, void *packed, int N, int K, hipStream_t s) {
+    QCHECK(N > 0 && N <= I8_MAX_N && K > 0 && K <= I8_MAX_K && ldw >= K, "%s: bad shape N=%d K=%d ldw=%d (N <= %d, K <= %d)", who, N, K, ldw, I8_MAX_N, I8_MAX_K);
     QCHECK(((uintptr_t)packed & 15) == 0, "%s: misaligned pointer", who);
-    const size_t total = (size_t)tiles * i8_ksteps(K) * 64;
+    const size_t total = (size_t)ceil_div(N, up ? 8 : 16) * i8_ksteps(K) * 64;
     hipLaunchKernelGGL(pack_int8_kernel, dim3((unsigned)std::min<size_t>((total + 255) / 256, 1 << 20)), dim3(256), 0, s,
                        (const int8_t *)w, (const int8_t *)up, ldw, (uint4 *)packed, N, K, i8_ksteps(K), total);
     QLAUNCH();
@@ -364,11 +375,11 @@ static int pack_int8(const char *who, const void *w, const void *up, int ldw, vo
 }
 extern "C" int qtts_pack_weight_int8(const void *w, int ldw, void *packed, int N, int K, qtts_stream_t stream) {
     QCHECK(w && packed, "pack_weight_int8: null pointer");
-    return pack_int8("pack_weight_int8", w, nullptr, ldw, packed, N, K, ceil_div(N, 16), (hipStream_t)stream);
+    return pack_int8("pack_weight_int8", w, nullptr, ldw, packed, N, K, (hipStream_t)stream);
 }
 extern "C" int qtts_pack_gate_up_int8(const void *gate, const void *up, int ldw, void *packed, int I, int K, qtts_stream_t stream) {
     QCHECK(gate && up && packed, "pack_gate_up_int8: null pointer");
-    return pack_int8("pack_gate_up_int8", gate, up, ldw, packed, I, K, ceil_div(I, 8), (hipStream_t)stream);
+    return pack_int8("pack_gate_up_int8", gate, up, ldw, packed, I, K, (hipStream_t)stream);
 }
 
 // ------------------------------------------------------------------ the product
@@ -878,9 +889,11 @@ static int linear_int8_checked(const char *who, const void *x, int ldx, const fl
                                const float *us, const void *bias, const void *res, int ldr, void *out, int ldo, int M, int N,
                                int K, bool swiglu, qtts_stream_t stream) {
     QCHECK(x && xs && wp && ws && out && (!swiglu || us), "%s: null pointer", who);
-    QCHECK(M > 0 && N > 0 && K > 0 && K <= I8_MAX_K && N <= 0x3ffffff, "%s: bad shape M=%d N=%d K=%d (K <= %d)", who, M, N, K, I8_MAX_K);
+    QCHECK(M > 0 && M <= I8_MAX_ROWS && N > 0 && N <= I8_MAX_N && K > 0 && K <= I8_MAX_K, "%s: bad shape M=%d N=%d K=%d (M <= %d, N <= %d, K <= %d)", who, M, N, K,
+           I8_MAX_ROWS, I8_MAX_N, I8_MAX_K);
     QCHECK(ldx % 16 == 0 && ldx >= K, "%s: x row stride %d too small or not a multiple of 16", who, ldx);
     QCHECK(ldo >= N && (!res || ldr >= N), "%s: row strides ldo=%d ldr=%d < N=%d", who, ldo, ldr, N);
+    QCHECK(out != res || ldo == ldr, "%s: out in the place of the residual needs its row stride", who);
     QCHECK((((uintptr_t)x | (uintptr_t)wp) & 15) == 0 && (((uintptr_t)xs | (uintptr_t)ws | (uintptr_t)us) & 3) == 0 &&
            (((uintptr_t)out | (uintptr_t)bias | (uintptr_t)res) & 1) == 0, "%s: misaligned pointer", who);
     LinI8Args a{};

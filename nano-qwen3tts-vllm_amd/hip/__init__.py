@@ -108,7 +108,7 @@ def stream():
     return torch.cuda.current_stream().cuda_stream
 
 
-current_device = torch.cuda.current_device
+current_device = torch._C._cuda_getDevice        # torch.cuda.current_device for a process that has a device tensor already
 
 
 # ---------------------------------------------------------------- tensor-level wrappers
@@ -248,13 +248,13 @@ def _rows_of(t, dtype, what, dev, rows=None, cols=None):
 
 
 def _vector_of(t, dtype, what, dev, n):
-    if t.get_device() != dev or t.dtype is not dtype or t.shape != (n,) or (t.stride(0) != 1 and n > 1):
+    if t.get_device() != dev or t.dtype is not dtype or t.numel() != n or not t.is_contiguous():
         raise QttsError(f"{what}: need {n} contiguous {dtype} on device {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()
 
 
 def _packed_of(t, nbytes, what, dev):
-    if t.get_device() != dev or t.dtype is not torch.uint8 or t.shape != (nbytes,):
+    if t.get_device() != dev or t.dtype is not torch.uint8 or t.numel() != nbytes or not t.is_contiguous():
         raise QttsError(f"{what}: need the {nbytes} bytes that packing made for this shape, on device {dev}; got "
                         f"{tuple(t.shape)} {t.dtype} on {t.device}")
     return t.data_ptr()

@@ -24,7 +24,7 @@ def quantize(x=P, ldx=64, q=P, ldq=64, s=P, M=4, K=64):
 
 @pytest.mark.parametrize("kwargs,word", [
     (dict(x=None), "null"), (dict(q=None), "null"), (dict(s=None), "null"), (dict(M=0), "shape"), (dict(M=-3), "shape"),
-    (dict(K=0), "shape"), (dict(K=131072, ldx=131072, ldq=131072), "shape"), (dict(ldx=63), "strides"), (dict(ldq=48), "strides"),
+    (dict(K=0), "shape"), (dict(K=131072, ldx=131072, ldq=131072), "shape"), (dict(M=0x7f800001), "shape"), (dict(ldx=63), "strides"), (dict(ldq=48), "strides"),
     (dict(ldq=72), "strides"), (dict(x=P + 1), "misaligned"), (dict(q=P + 8), "misaligned"), (dict(s=P + 2), "misaligned"),
 ])
 def test_quantize_refuses(kwargs, word):
@@ -37,7 +37,8 @@ def rmsnorm(x=P, ldx=64, d=P, ldd=64, w=P, sm=P, lds=64, q=P, ldq=64, s=P, M=4, 
 
 @pytest.mark.parametrize("kwargs,word", [
     (dict(x=None), "null"), (dict(w=None), "null"), (dict(q=None), "null"), (dict(s=None), "null"), (dict(d=None), "come together"),
-    (dict(sm=None), "come together"), (dict(M=0), "shape"), (dict(H=0), "shape"), (dict(H=131072, ldx=1 << 18, ldd=1 << 18, lds=1 << 18,
+    (dict(sm=None), "come together"), (dict(M=0), "shape"), (dict(M=0x7fffffff), "shape"), (dict(ldx=72, d=P + 4096, lds=64), "in the place of x"),
+    (dict(x=P + 4096, ldd=72), "in the place of x or delta"), (dict(H=0), "shape"), (dict(H=131072, ldx=1 << 18, ldd=1 << 18, lds=1 << 18,
     ldq=1 << 18), "shape"), (dict(ldx=60), "strides"), (dict(ldd=60), "strides"), (dict(lds=60), "strides"), (dict(ldq=60), "strides"),
     (dict(ldq=72), "strides"), (dict(x=P + 1), "misaligned"), (dict(d=P + 1), "misaligned"), (dict(w=P + 1), "misaligned"),
     (dict(sm=P + 1), "misaligned"), (dict(q=P + 4), "misaligned"), (dict(s=P + 1), "misaligned"),
@@ -53,6 +54,7 @@ def linear(x=P, ldx=64, xs=P, w=P, ws=P, b=None, r=None, ldr=0, out=P, ldo=32, M
 @pytest.mark.parametrize("kwargs,word", [
     (dict(x=None), "null"), (dict(xs=None), "null"), (dict(w=None), "null"), (dict(ws=None), "null"), (dict(out=None), "null"),
     (dict(M=0), "shape"), (dict(N=0), "shape"), (dict(K=0), "shape"), (dict(K=131072, ldx=131072), "shape"), (dict(N=-1), "shape"),
+    (dict(M=0x7f800001), "shape"), (dict(N=0x4000000, ldo=0x4000000), "shape"), (dict(r=P, ldr=40), "in the place of the residual"),
     (dict(ldx=48), "row stride"), (dict(ldx=72), "row stride"), (dict(ldo=31), "strides"), (dict(r=P, ldr=31), "strides"),
     (dict(x=P + 8), "misaligned"), (dict(w=P + 8), "misaligned"), (dict(xs=P + 2), "misaligned"), (dict(ws=P + 2), "misaligned"),
     (dict(out=P + 1), "misaligned"), (dict(b=P + 1), "misaligned"), (dict(r=P + 1, ldr=32), "misaligned"),
@@ -79,6 +81,7 @@ def test_packing_refuses_and_sizes():
     refuses(L.qtts_pack_weight_int8(P, 63, P, 16, 64, None), "pack_weight_int8:", "shape")
     refuses(L.qtts_pack_weight_int8(P, 1 << 18, P, 16, 131072, None), "pack_weight_int8:", "shape")
     refuses(L.qtts_pack_weight_int8(P, 64, P + 8, 16, 64, None), "pack_weight_int8:", "misaligned")
+    refuses(L.qtts_pack_weight_int8(P, 64, P, 0x4000000, 64, None), "pack_weight_int8:", "shape")
     refuses(L.qtts_pack_gate_up_int8(P, None, 64, P, 16, 64, None), "pack_gate_up_int8:", "null")
     refuses(L.qtts_pack_gate_up_int8(P, P, 64, P, 0, 64, None), "pack_gate_up_int8:", "shape")
     assert L.qtts_packed_weight_int8_bytes(16, 128) == 2048 and L.qtts_packed_weight_int8_bytes(17, 129) == 2 * 2 * 2048
