@@ -112,7 +112,8 @@ int qtts_linear_swiglu_fp8(const void *x, int ldx, const void *w_gate_up_fp8_pac
  * qtts_quantize_int8: scales[m] = max(max|x[m]| / 127, 2^-126), q[m] = rint(x[m] / scales[m]), |q| <= 127.
  * (Also quantises F.linear weights [N,K] per output channel, for qtts_pack_weight_int8.)
  * qtts_rmsnorm_int8: h = bf16(x + delta) is written to `sum` (which may be x or delta itself, with its stride); then
- * y = h / sqrt(mean(h^2) + eps) * w in fp32, not rounded in between, quantised as above.  delta == sum == NULL: h = x.
+ * y = h / sqrt(mean(h^2) + eps) * w in fp32 (the mean too: it overflows where sum(h^2) does), not rounded in between,
+ * quantised as above.  delta == sum == NULL: h = x.
  * The norm of P/layers/layernorm.py:17-27 behind the residual addition of P/models/qwen3_tts_share.py:171,175. */
 int qtts_quantize_int8(const void *x, int ldx, void *q, int ldq, float *scales, int M, int K, qtts_stream_t stream);
 int qtts_rmsnorm_int8(const void *x, int ldx, const void *delta, int ldd, const void *w, float eps, void *sum, int lds,

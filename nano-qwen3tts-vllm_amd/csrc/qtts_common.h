@@ -1,7 +1,7 @@
 // qtts_common.h - what the translation units of libqtts_hip share: error reporting, the bf16 / lane helpers every
 // kernel uses, the activation layouts, the dispatch thresholds, the GEMM launcher's argument record and the few
-// host functions one unit calls in another (gemm: qtts_gemm.hip, attention: qtts_attention.hip, sampling and the
-// per-frame glue: qtts_glue.hip, the decoder stack and graphs: qtts_model.hip).
+// host functions one unit calls in another (gemm: qtts_gemm.hip, 8-bit integers: qtts_int8.hip, attention:
+// qtts_attention.hip, sampling and the per-frame glue: qtts_glue.hip, the decoder stack and graphs: qtts_model.hip).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
@@ -79,8 +79,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
 }
 
 // RMSNorm of two neighbouring elements (one dword of bf16 pairs): bf16(bf16(x * rstd) * w), the reference's rounding
-// points (P/layers/layernorm.py:17-27), on the packed fp32 multiplier and the packed fp32 -> bf16 conversion (half the
-// instructions of the element-by-element form, same bits).
+// points (P/layers/layernorm.py:17-27), on the packed fp32 -> bf16 conversion (same bits as element by element).
 typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t pack2v(float2_t v) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, bf16x2_t));       // v_cvt_pk_bf16_f32: RNE

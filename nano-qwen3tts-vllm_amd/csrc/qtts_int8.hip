@@ -93,6 +93,9 @@ __device__ __forceinline__ void store8_i8(int8_t *row, int k0, int K, float (&v)
 // A row per T = 64 * W threads, R rows a workgroup; thread t of a row holds the 8-column chunks t, t + T, ... (CH of them) as
 // bf16 across both reductions, so x, delta and the weights are read once and nothing is read back.  All of a thread's
 // requests go out before its first store: sum may be x or delta, and a load behind a store that may alias waits for it.
+// Few rows are bound by the chain request - sum of squares - maximum - store (8 rows of 2048 with delta 3.6 us, an empty launch
+// 2.3), many by memory: 16384 x 2048 with delta 44.3 us, 5.3 TB/s of the 4.9-5.4 a large copy reaches; 8192 x 6144 quantised
+// alone 24.3 us, 6.2 TB/s (part of what it reads is in the caches still).
 template <int W, int R, int CH, bool NORM>
 __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
     constexpr int T = W * 64;
@@ -206,7 +209,8 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 }
 
 // Rows too long for registers: three walks over the row, the second and third of them out of L2 - h is read back from where
-// the first walk wrote it (sum), or from x.  300 rows of 40000 columns: see launch_rows_int8.
+// the first walk wrote it (sum), or from x.  Bound by those walks' latencies, a workgroup a row: 300 rows of 40000 columns 12 us
+// quantised, 36 us with norm and delta (the form above, whose chunks such rows push out of the registers: 94 us).
 template <bool NORM>
 __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
     __shared__ float red_f[16];
@@ -333,6 +337,7 @@ extern "C" int qtts_rmsnorm_int8(const void *x, int ldx, const void *delta, int 
 }
 
 // ------------------------------------------------------------------ weight packing
+// Once per weight, at load time: a byte at a time is fast enough (bound by those loads).
 // packed[tile][k-step][lane][16 B]: lane (g, r) of k-step ks holds row 16 * tile + r, columns 64 * ks + 16 * g .. +16 - the
 // 16 bytes a lane feeds to v_mfma_i32_16x16x64_i8.  Rows and columns behind the last are zeros; k-steps come in pairs.
 // gate/up: the tile's packed row 4 * p + j holds output i = 8 * tile + 2 * p + (j & 1), gate for j < 2 and up for j >= 2: a
@@ -443,7 +448,10 @@ union I8Frag { uint4 u; int4_t v; };
 
 // Few rows: a workgroup owns TM row tiles x TN weight tiles and its NW waves share K, each wave a contiguous run of
 // k-steps straight from memory to registers; the waves' sums meet in LDS.  U k-steps are requested at a time, the next U
-// before the current are multiplied.
+// before the current are multiplied.  Every weight byte is used 16 TM times at most, so what bounds it is weights coming in:
+// the launch and one latency (1 row x 4096 x 2048: 3.8 us), then the 40-60 GB/s a CU takes of row-major activations and
+// weights together (16 x 2048 x 6144 with residual 7.5 us; SwiGLU 8 x 6144 x 2048 6.7 us, 3.8 TB/s).  Sixteen waves a
+// workgroup, or the epilogue's scales requested in front of the loop, are no faster.
 template <int TM, int TN, int NW, int U, bool SWIGLU>
 __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a) {
     __shared__ int4_t red[NW][TM * TN][64];
@@ -526,6 +534,11 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 // of them are on their way while one is multiplied.  The weights keep their fragment order; the rows of a 1 KiB request (16
 // rows x 64 columns or 8 x 128) stay row-major, the 16-byte chunk c of row r at place c ^ swizzle(r), so that the 16 rows a
 // fragment read touches lie in 16 different places modulo 256 bytes.
+// Small tiles are bound by LDS: 64 x 64 moves 48 KB through it per 128 columns, 384 of the 470 cycles these take (more stages,
+// or eight waves, change nothing; 200 x 4096 x 2048 8.0 us).  The largest tile is bound by the matrix units' power: 16384 x 2048 x
+// 6144 in 168-178 us, 2.3-2.4 POPS (the library's product 175-179), at 1.93 GHz - with zeros for data 136 us.  The 32 x 32 x 32
+// instruction, more stages, and fragments read a step ahead into registers are not faster there (186, 168 and 168 us where
+// this form took 168); without the turns of the two waves of a SIMD (ALT) it takes 183.
 template <int KS>
 __device__ __forceinline__ int i8_swizzle(int r) {
     // A 16-byte read is served 16 lanes at a time: 0-3, 12-15, 20-23, 24-27, then 4-7, 8-11, 16-19, 28-31, and so on.  With
@@ -823,7 +836,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 //   us = launch + (fixed + step * ceil(K / 64)) * load,   load = max(1, r + 3/4 (ceil(r) - r)),  r = workgroups / 256
 // fitted to the times of every form over 1-8192 rows and nine N x K from 1024 x 1024 to 8192 x 512 (cold weights, in a graph).
 // The form with the smallest estimate is taken: over those 261 shapes 0.8 % slower on average than the fastest form of each, at
-// most 14 %.  Some of them (us of the forms in the table's order, '-' far off):
+// most 14 %; over 60 shapes drawn at random that the fit had not seen, the same.  Some of them (us of the forms in the table's order, '-' far off):
 //   1 x 4096 x 2048 (plain)       3.9  3.9  4.2  4.8  5.5  6.8   -    -    -    -
 //   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   16   -    -    -    -
 //   200 x 4096 x 2048 (plain)      17   17   12   12   11  7.9   13   13   17   26

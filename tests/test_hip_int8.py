@@ -127,7 +127,7 @@ def test_rows_with_other_strides_and_alignments(hip, off, ld):
 
 
 @pytest.mark.parametrize("into", ["x", "delta"])
-@pytest.mark.parametrize("H", [512, 2047, 5000])
+@pytest.mark.parametrize("H", [512, 2047, 5000, 20001])
 def test_rmsnorm_sum_in_place(hip, into, H):
     g = gen(4, H)
     x, d, w = rand_bf16(g, 5, H), rand_bf16(g, 5, H), rand_bf16(g, H)
