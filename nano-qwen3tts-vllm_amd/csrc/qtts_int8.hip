@@ -517,6 +517,56 @@ __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a)
     }
 }
 
+// Few rows and few columns: 8 rows and half a packed tile a workgroup, so that twice as many CUs take part.  An instruction takes
+// two k-steps: its weight rows 0-7 and activation rows 0-7 are a step's, 8-15 the same rows of the next; of the four quarters
+// of its sums two are wanted, and added up.  Bound by latency, then by what a CU takes in: 8 x 2048 x 6144 5.6 us (6.2 in
+// whole tiles, whose activations are requested for 16 rows), 8 x 512 x 8192 5.0 us (5.8), 16 x 512 x 8192 5.1 us (7.0); 16 rows
+// of whole steps to half a tile, other U (1, 3, 4) and four or sixteen waves are slower on most shapes.
+template <int NW, int U, bool SWIGLU>
+__global__ __launch_bounds__(NW * 64) void linear_int8_half_kernel(LinI8Args a) {
+    __shared__ int4_t red[NW][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = lane & 15, g = lane >> 4;
+    const int tile = blockIdx.x >> 1, half = blockIdx.x & 1, m = blockIdx.y * 8 + (r & 7), odd = r >> 3;
+    const int pairs = ceil_div(a.K, 128), per = ceil_div(pairs, NW), p0 = min(pairs, wave * per), n = min(pairs, p0 + per) - p0;
+    const int8_t *xp = a.x + (size_t)min(m, a.M - 1) * a.ldx;
+    const uint4 *wp = a.wp + (size_t)tile * a.ksteps * 64 + 16 * g + 8 * half + (r & 7);
+    int4_t acc = {0, 0, 0, 0};
+    struct Batch { I8Frag x[U], w[U]; } b0, b1;
+    auto request = [&](Batch &b, int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int ks = 2 * (p0 + min(at + u, n - 1)) + odd;                     // behind the run: its last pair again, not multiplied
+            const int k = 64 * ks + 16 * g, kk = k < a.K ? k : 0;                    // behind the last column the packed weights are zeros
+            b.x[u].u = *reinterpret_cast<const uint4 *>(xp + kk);
+            b.w[u].u = wp[(size_t)ks * 64];
+        }
+    };
+    auto multiply = [&](const Batch &b, int at) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            if (at + u >= n) break;
+            acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(b.w[u].v, b.x[u].v, acc, 0, 0, 0);
+        }
+    };
+    if (n > 0) {
+        request(b0, 0);
+        for (int at = 0; at < n; at += 2 * U) {
+            if (at + U < n) request(b1, at + U);
+            multiply(b0, at);
+            if (at + U >= n) break;
+            if (at + 2 * U < n) request(b0, at + 2 * U);
+            multiply(b1, at + U);
+        }
+    }
+    red[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0 || g > 1 || r > 7) return;
+    int4_t sum = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < NW; ++w) sum += red[w][lane] + red[w][lane + 40];            // weight row + 8, activation row + 8
+    i8_store<SWIGLU>(a, sum, tile, m, lane + 32 * half);
+}
+
 #pragma clang diagnostic ignored "-Winline-asm"     // "reserved register" m0 in a clobber list: it is what the block writes
 // 16 bytes per lane from memory to LDS, lane i's to place i behind the LDS address `at` (the same in every lane).  In
 // assembly because the compiler, which sees a write to LDS in the builtin, waits for it in front of the next read of any
@@ -835,13 +885,15 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 // launch's is that times the workgroups a CU gets, on top of what the launch itself takes:
 //   us = launch + (fixed + step * ceil(K / 64)) * load,   load = max(1, r + 3/4 (ceil(r) - r)),  r = workgroups / 256
 // fitted to the times of every form over 1-8192 rows and nine N x K from 1024 x 1024 to 8192 x 512 (cold weights, in a graph).
-// The form with the smallest estimate is taken: over those 261 shapes 0.8 % slower on average than the fastest form of each, at
-// most 14 %; over 60 shapes drawn at random that the fit had not seen, the same.  Some of them (us of the forms in the table's order, '-' far off):
-//   1 x 4096 x 2048 (plain)       3.9  3.9  4.2  4.8  5.5  6.8   -    -    -    -
-//   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   16   -    -    -    -
-//   200 x 4096 x 2048 (plain)      17   17   12   12   11  7.9   13   13   17   26
-//   800 x 4096 x 2048 (plain)       -    -    -    -    -   20   15   14   18   29
-//   4096 x 4096 x 2048 (plain)      -    -    -    -    -   65   44   50   41   38
+// The form with the smallest estimate is taken: 1 % slower on average than the fastest form of each shape over those and over
+// 102 others that the fit had not seen (60 drawn at random, 42 with few columns), at most 16 %.  Some of them (us of the forms
+// in the table's order, '-' far off):
+//   1 x 4096 x 2048 (plain)       4.0  3.9  4.1  4.7  5.4  4.0  7.7   -    -    -    -
+//   8 x 2048 x 6144 (plain)       7.6  6.2  8.0  8.1   12  5.6   17   -    -    -    -
+//   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   16   16   -    -    -    -
+//   200 x 4096 x 2048 (plain)      17   17   12   12   11   -   7.9   13   13   17   26
+//   800 x 4096 x 2048 (plain)       -    -    -    -    -   -    20   15   14   18   29
+//   4096 x 4096 x 2048 (plain)      -    -    -    -    -   -    65   44   50   41   38
 struct I8Form { int bm, bn; float launch, fixed, step; };
 static constexpr I8Form I8_FORMS[] = {
     {16, 16, 2.52f, 0.117f, 0.037f},     // K over 4 waves
@@ -849,13 +901,14 @@ static constexpr I8Form I8_FORMS[] = {
     {16, 32, 2.42f, 0.147f, 0.048f},     // over 4
     {32, 32, 2.04f, 0.565f, 0.073f},     // over 8
     {32, 64, 1.84f, 1.029f, 0.109f},     // over 8
+    {8, 8, 2.48f, 0.201f, 0.019f},       // half a packed tile, over 8
     {64, 64, 3.50f, 0.409f, 0.112f},     // through LDS, as the rest
     {128, 128, 3.97f, 1.346f, 0.279f},
     {128, 128, 1.57f, 3.497f, 0.280f},   // two k-steps a stage, waves in turns
     {128, 256, 0.94f, 6.138f, 0.387f},   // the same
     {256, 256, 0.04f, 11.115f, 0.670f},  // one k-step a stage, waves in turns
 };
-static constexpr int I8_SPLIT_FORMS = 5;
+static constexpr int I8_SPLIT_FORMS = 6;
 #ifdef QTTS_TUNING
 static int g_i8_form = -1;
 extern "C" void qtts_tune_int8(int form) { g_i8_form = form; }      // measurement builds: this form whatever the shape
@@ -869,7 +922,8 @@ static int choose_int8_form(int M, int columns, int K) {
     double least = 0;
     for (int f = 0; f < (int)(sizeof(I8_FORMS) / sizeof(I8_FORMS[0])); ++f) {
         const I8Form &F = I8_FORMS[f];
-        if (f < I8_SPLIT_FORMS && ceil_div(M, F.bm) > 65535) continue;              // the row blocks are blockIdx.y there
+        // these take a workgroup per tile: row blocks are blockIdx.y, and a row of blocks takes fewer than 2^32 threads
+        if (f < I8_SPLIT_FORMS && (ceil_div(M, F.bm) > 65535 || ceil_div(columns, F.bn) > 1 << 22)) continue;
         const double r = (double)ceil_div(M, F.bm) * ceil_div(columns, F.bn) / 256;
         const double us = F.launch + (F.fixed + F.step * ceil_div(K, 64)) * std::max(1.0, 0.25 * r + 0.75 * ceil(r));
         if (best < 0 || us < least) { best = f; least = us; }
@@ -890,11 +944,12 @@ static void launch_int8_form(const LinI8Args &a, int tiles, int form, hipStream_
     case 2: QTTS_SPLIT_I8(1, 2, 4, 4); break;
     case 3: QTTS_SPLIT_I8(2, 2, 8, 2); break;
     case 4: QTTS_SPLIT_I8(2, 4, 8, 2); break;
-    case 5: QTTS_TILE_I8(64, 64, 2, 2, 2, 4, false, 2); break;
-    case 6: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, false, 2); break;
-    case 7: QTTS_TILE_I8(128, 128, 2, 4, 2, 4, true, 1); break;
-    case 8: QTTS_TILE_I8(128, 256, 2, 4, 2, 3, true, 1); break;
-    case 9: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, true, 1); break;
+    case 5: hipLaunchKernelGGL((linear_int8_half_kernel<8, 2, SWIGLU>), dim3(ceil_div(a.N, SWIGLU ? 4 : 8), ceil_div(a.M, 8)), dim3(512), 0, s, a); break;
+    case 6: QTTS_TILE_I8(64, 64, 2, 2, 2, 4, false, 2); break;
+    case 7: QTTS_TILE_I8(128, 128, 2, 4, 1, 4, false, 2); break;
+    case 8: QTTS_TILE_I8(128, 128, 2, 4, 2, 4, true, 1); break;
+    case 9: QTTS_TILE_I8(128, 256, 2, 4, 2, 3, true, 1); break;
+    case 10: QTTS_TILE_I8(256, 256, 2, 4, 1, 4, true, 1); break;
     }
 #undef QTTS_TILE_I8
 #undef QTTS_SPLIT_I8

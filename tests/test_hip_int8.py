@@ -235,7 +235,7 @@ def check_product(got, x, xs, w, ws, b=None, r=None):
     assert float(off.max()) <= 0, (float(off.max()), (off > 0).nonzero()[:4].tolist())
 
 
-PRODUCTS = [(1, 1, 1), (1, 16, 64), (1, 4096, 2048), (2, 100, 33), (7, 1000, 200), (8, 2048, 6144), (15, 48, 4097), (16, 2048, 2048),
+PRODUCTS = [(1, 1, 1), (1, 16, 64), (1, 4096, 2048), (2, 100, 33), (8, 4, 300), (9, 13, 8000), (20, 9, 1025), (300, 7, 2000), (6, 2043, 2049), (7, 1000, 200), (8, 2048, 6144), (15, 48, 4097), (16, 2048, 2048),
             (17, 250, 129), (33, 512, 512), (48, 1000, 1111), (64, 4096, 1024), (65, 77, 6000), (100, 2050, 300), (128, 128, 128),
             (129, 257, 640), (200, 4096, 2048), (255, 511, 96), (257, 300, 1025), (500, 1000, 1000), (777, 1000, 1111), (1000, 64, 5000),
             (1025, 2047, 257), (2048, 2048, 512), (3000, 24, 24), (4100, 1030, 130)]
@@ -278,7 +278,7 @@ def swiglu_case(hip, M, I, K):
     return x, xs, gate, gs, up, us
 
 
-@pytest.mark.parametrize("M,I,K", [(1, 1, 1), (1, 6144, 2048), (3, 100, 33), (8, 6144, 2048), (16, 1023, 512), (17, 8, 64), (40, 250, 129),
+@pytest.mark.parametrize("M,I,K", [(1, 1, 1), (1, 6144, 2048), (3, 100, 33), (8, 3, 500), (5, 1021, 2100), (8, 6144, 2048), (16, 1023, 512), (17, 8, 64), (40, 250, 129),
                                    (64, 2048, 1024), (100, 1001, 300), (130, 70, 2000), (200, 6144, 2048), (300, 129, 640),
                                    (513, 1000, 1111), (1030, 2047, 96), (2048, 1024, 512), (4100, 515, 130)])
 def test_linear_swiglu(hip, M, I, K):
