@@ -584,8 +584,10 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 // of them are on their way while one is multiplied.  The weights keep their fragment order; the rows of a 1 KiB request (16
 // rows x 64 columns or 8 x 128) stay row-major, the 16-byte chunk c of row r at place c ^ swizzle(r), so that the 16 rows a
 // fragment read touches lie in 16 different places modulo 256 bytes.
-// Small tiles are bound by LDS: 64 x 64 moves 48 KB through it per 128 columns, 384 of the 470 cycles these take (more stages,
-// or eight waves, change nothing; 200 x 4096 x 2048 8.0 us).  The largest tile is bound by the matrix units' power: 16384 x 2048 x
+// Small tiles are bound by what comes in: 64 x 64 takes 0.29 us per 128 columns, 0.23 of them for the requests alone (16 KB,
+// 70 GB/s a CU; rows that all lie in L2 would come at 130) and 0.18 for LDS reads and products alone (200 x 4096 x 2048 8.1 us,
+// 200 x 2048 x 6144 in 32 x 64 tiles above 13 us).  More stages, eight waves, fragments read a step ahead, padded rows and a
+// start along K that differs between workgroups change nothing or cost 2-9 %.  The largest tile is bound by the matrix units' power: 16384 x 2048 x
 // 6144 in 168-178 us, 2.3-2.4 POPS (the library's product 175-179), at 1.93 GHz - with zeros for data 136 us.  The 32 x 32 x 32
 // instruction, more stages, and fragments read a step ahead into registers are not faster there (186, 168 and 168 us where
 // this form took 168); without the turns of the two waves of a SIMD (ALT) it takes 183.
@@ -890,7 +892,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 // in the table's order, '-' far off):
 //   1 x 4096 x 2048 (plain)       4.0  3.9  4.1  4.7  5.4  4.0  7.7   -    -    -    -
 //   8 x 2048 x 6144 (plain)       7.6  6.2  8.0  8.1   12  5.6   17   -    -    -    -
-//   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   16   16   -    -    -    -
+//   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   20   17   -    -    -    -
 //   200 x 4096 x 2048 (plain)      17   17   12   12   11   -   7.9   13   13   17   26
 //   800 x 4096 x 2048 (plain)       -    -    -    -    -   -    20   15   14   18   29
 //   4096 x 4096 x 2048 (plain)      -    -    -    -    -   -    65   44   50   41   38
