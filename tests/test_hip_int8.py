@@ -361,6 +361,35 @@ def test_offsets_beyond_32_bits(hip):
     check_product(out[-70:], q[-70:], s[-70:], wn, ws)
 
 
+@pytest.mark.parametrize("M,K", [((1 << 22) + 9, 8), ((1 << 20) + 5, 520)])
+def test_more_rows_than_workgroups_of_a_launch(hip, M, K):
+    """Workgroups take several rows each: the last rows equal the same rows computed alone."""
+    g = gen(31, K)
+    x, w = rand_bf16(g, M, K), rand_bf16(g, K)
+    d = x.flip(0)
+    for got, alone in ((hip.quantize_int8(x), hip.quantize_int8(x[-40:])),
+                       (hip.rmsnorm_int8(x, w, 1e-6, delta=d), hip.rmsnorm_int8(x[-40:], w, 1e-6, delta=d[-40:]))):
+        for a, b in zip(got, alone):
+            assert torch.equal(a[-40:], b)
+    q, s = hip.quantize_int8(x)
+    check = torch.arange(0, M, 4099, device=DEV)
+    for a, b in zip((q, s), hip.quantize_int8(x[check])):
+        assert torch.equal(a[check], b)
+
+
+@pytest.mark.parametrize("M", [600_001, 1_100_000, 2_200_000])
+def test_more_rows_than_a_grid_is_high(hip, M):
+    """Row blocks of the forms for few columns pass 65535: forms with larger blocks are taken."""
+    N, K = 3, 16
+    x, xs, w, ws, b, r = product_case(hip, M, N, K, True, True)
+    check_product(hip.linear_int8(x, xs, hip.pack_weight_int8(w), ws, N, bias=b, residual=r), x, xs, w, ws, b, r)
+    up, us = w.flip(0).contiguous(), ws.flip(0).contiguous()
+    pg = hip.pack_gate_up_int8(w, up)
+    got = hip.linear_swiglu_int8(x, xs, pg, ws, us, N)
+    for at in (0, M // 2, M - 50):
+        assert torch.equal(got[at:at + 50], hip.linear_swiglu_int8(x[at:at + 50], xs[at:at + 50].clone(), pg, ws, us, N))
+
+
 # ---------------------------------------------------------------- a run of them, as an MLP makes it
 def mlp_weights(hip, H, I, seed):
     g = gen(17, seed)
