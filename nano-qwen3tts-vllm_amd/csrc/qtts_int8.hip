@@ -886,8 +886,10 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 // A workgroup's time is a fixed part and a part per k-step, the bytes its CU pulls in at 50-70 GB/s (few bytes: latency); a
 // launch's is that times the workgroups a CU gets, on top of what the launch itself takes:
 //   us = launch + (fixed + step * ceil(K / 64)) * load,   load = max(1, r + 3/4 (ceil(r) - r)),  r = workgroups / 256
-// fitted to the times of every form over 1-8192 rows and nine N x K from 1024 x 1024 to 8192 x 512 (cold weights, in a graph).
-// The form with the smallest estimate is taken: 1 % slower on average than the fastest form of each shape over those and over
+// but no less than the weights take from memory at 6 TB/s, times ceil(r) / r for the CUs that idle at the end or throughout
+// (2.4 at most: that is what a CU takes alone; SwiGLU 8 x 6144 x 2048 7.4 us in the form chosen without this, 6.8 with it).  The
+// table is fitted to the times of every form over 1-8192 rows and nine N x K from 1024 x 1024 to 8192 x 512 (cold weights, in
+// a graph).  The form with the smallest estimate is taken: 1 % slower on average than the fastest form of each shape, 2 % over
 // 102 others that the fit had not seen (60 drawn at random, 42 with few columns), at most 16 %.  Some of them (us of the forms
 // in the table's order, '-' far off):
 //   1 x 4096 x 2048 (plain)       4.0  3.9  4.1  4.7  5.4  4.0  7.7   -    -    -    -
@@ -927,7 +929,8 @@ static int choose_int8_form(int M, int columns, int K) {
         // these take a workgroup per tile: row blocks are blockIdx.y, and a row of blocks takes fewer than 2^32 threads
         if (f < I8_SPLIT_FORMS && (ceil_div(M, F.bm) > 65535 || ceil_div(columns, F.bn) > 1 << 22)) continue;
         const double r = (double)ceil_div(M, F.bm) * ceil_div(columns, F.bn) / 256;
-        const double us = F.launch + (F.fixed + F.step * ceil_div(K, 64)) * std::max(1.0, 0.25 * r + 0.75 * ceil(r));
+        const double cu = (F.fixed + F.step * ceil_div(K, 64)) * std::max(1.0, 0.25 * r + 0.75 * ceil(r));
+        const double us = F.launch + std::max(cu, 64.0 * columns * ceil_div(K, 64) / 6e6 * std::min(2.4, ceil(r) / r));
         if (best < 0 || us < least) { best = f; least = us; }
     }
     return best;

@@ -19,6 +19,7 @@ from nano_qwen3tts_vllm import hip  # noqa: E402
 _p, _i = C.c_void_p, C.c_int
 for _name, (_res, _args) in {
     "qtts_tune_linear": (None, [_i, _i]),
+    "qtts_tune_int8": (None, [_i]),
     "qtts_tune_subtiles": (None, [_i]),
     "qtts_tune_prompt_attention": (None, [_i]),
     "qtts_tune_rows": (None, [_i]),

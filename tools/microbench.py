@@ -678,6 +678,76 @@ def prefill():
         print(f"prefill {plen:4d} tokens: " + " ".join(f"{v:.2f}" for v in ts) + " ms", flush=True)
 
 
+def int8():
+    """The 8-bit operators inside a graph, weights cold: a product in the form the library chooses and in each of the
+    others, rows with a scale each, and the MLP block of them."""
+    R = 24
+    rnd = lambda *shape: torch.randint(-127, 128, shape, device=dev, dtype=torch.int8)   # noqa: E731
+
+    def graph_us(fn, n=R):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            fn(0)
+            g = hip.Graph.capture(lambda: [fn(i) for i in range(n)])
+        return timed(lambda: g.launch(), n)
+
+    for what, M, N, K in (("linear", 1, 4096, 2048), ("linear", 8, 2048, 6144), ("linear+res", 16, 2048, 6144), ("linear", 200, 4096, 2048),
+                          ("linear+res", 777, 1000, 1111), ("linear+res", 16384, 2048, 6144), ("swiglu", 8, 6144, 2048),
+                          ("swiglu", 200, 6144, 2048), ("swiglu", 8192, 6144, 2048)):
+        two = what == "swiglu"
+        nbuf = max(1, min(60, int(600e6 // (N * K * (1 + two)))))
+        x = hip.int8_rows(M, K, dev)
+        x.copy_(rnd(M, K))
+        xs, ws = torch.rand(M, device=dev), torch.rand(N, device=dev) * 1e-4
+        wp = [hip.pack_gate_up_int8(rnd(N, K), rnd(N, K)) if two else hip.pack_weight_int8(rnd(N, K)) for _ in range(nbuf)]
+        out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+        res = torch.randn(M, N, device=dev).bfloat16() if what == "linear+res" else None
+
+        def run(i):
+            if two:
+                hip.linear_swiglu_int8(x, xs, wp[i % nbuf], ws, ws, N, out=out)
+            else:
+                hip.linear_int8(x, xs, wp[i % nbuf], ws, N, residual=res, out=out)
+
+        n = R if M < 1000 else 4
+        us = []
+        for form in (*range(11), -1):                    # -1: the library's choice
+            hip.lib.qtts_tune_int8(form)
+            us.append(graph_us(run, n))
+        ops = 2 * M * N * K * (1 + two)
+        print(f"{what:10s} {M:5d} x {N} x {K}: {us[-1]:6.1f} us {ops / us[-1] / 1e6:5.0f} TOPS   forms " + " ".join(f"{u:.1f}" for u in us[:-1]),
+              flush=True)
+    for what, M, K in (("rmsnorm", 8, 2048), ("rmsnorm", 16384, 2048), ("quantize", 333, 1111), ("quantize", 8192, 6144)):
+        x, d, w = (torch.randn(*s, device=dev).bfloat16() for s in ((M, K), (M, K), (K,)))
+        h, q, s = torch.empty_like(x), hip.int8_rows(M, K, dev), torch.empty(M, device=dev)
+        if what == "rmsnorm":
+            us, by = graph_us(lambda i: hip.rmsnorm_int8(x, w, delta=d, sum_out=h, out=q, scales=s)), 7 * M * K
+        else:
+            us, by = graph_us(lambda i: hip.quantize_int8(x, out=q, scales=s)), 3 * M * K
+        print(f"{what:10s} {M:5d} x {K}: {us:6.1f} us {by / us / 1e6:5.2f} TB/s", flush=True)
+    H, I = 2048, 6144
+    q = lambda n, k: hip.quantize_int8((torch.randn(n, k, device=dev) * k ** -0.5).bfloat16())   # noqa: E731
+    nbuf = 16
+    mlps = []
+    for _ in range(nbuf):
+        (g, gs), (u, us), (d, ds) = q(I, H), q(I, H), q(H, I)
+        mlps.append((hip.pack_gate_up_int8(g, u), gs, us, hip.pack_weight_int8(d), ds))
+    nw = torch.ones(H, device=dev).bfloat16()
+    for M in (1, 8, 64, 200, 1024, 4096, 16384):
+        x, d = torch.randn(M, H, device=dev).bfloat16(), torch.randn(M, H, device=dev).bfloat16()
+        h, o, a = torch.empty_like(x), torch.empty_like(x), torch.empty(M, I, device=dev, dtype=torch.bfloat16)
+        xq, xs, aq, as_ = hip.int8_rows(M, H, dev), torch.empty(M, device=dev), hip.int8_rows(M, I, dev), torch.empty(M, device=dev)
+
+        def block(i):
+            gu, gs, us, dn, ds = mlps[i % nbuf]
+            hip.rmsnorm_int8(x, nw, delta=d, sum_out=h, out=xq, scales=xs)
+            hip.linear_swiglu_int8(xq, xs, gu, gs, us, I, out=a)
+            hip.quantize_int8(a, out=aq, scales=as_)
+            hip.linear_int8(aq, as_, dn, ds, H, residual=h, out=o)
+
+        print(f"MLP block  {M:5d} rows: {graph_us(block, nbuf):6.1f} us", flush=True)
+
+
 if __name__ == "__main__":
     _tuning.apply_env_flags()
-    {"prefill": prefill, "prefill_batch": prefill_batch, "decode_eager": decode_eager, "rows": rows, "rowsn": rowsn, "attn": attn, "attntrace": attntrace, "rowtrace": rowtrace, "launch": launch, "linear": linear, "linear2": linear2, "frame": frame, "dominant": dominant, "lat": lat, "mall": mall, "gridbar": gridbar, "trace": trace}[sys.argv[1]]()
+    {"prefill": prefill, "prefill_batch": prefill_batch, "decode_eager": decode_eager, "rows": rows, "rowsn": rowsn, "attn": attn, "attntrace": attntrace, "rowtrace": rowtrace, "launch": launch, "linear": linear, "linear2": linear2, "frame": frame, "dominant": dominant, "lat": lat, "mall": mall, "gridbar": gridbar, "trace": trace, "int8": int8}[sys.argv[1]]()
