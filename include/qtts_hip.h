@@ -109,7 +109,8 @@ int qtts_linear_swiglu_fp8(const void *x, int ldx, const void *w_gate_up_fp8_pac
  * the number of rows, nor on the rows beside it.  M <= 2139095040, N and I <= 67108863.  A row that holds a NaN or an
  * infinity gets a scale that is NaN or infinite and q = 0: everything computed from that row is NaN, no other row is touched.
  *
- * qtts_quantize_int8: scales[m] = max(max|x[m]| / 127, 2^-126), q[m] = rint(x[m] / scales[m]), |q| <= 127.
+ * qtts_quantize_int8: scales[m] = max(max|x[m]| / 127, 2^-126), q[m] = rint(x[m] / scales[m]), |q| <= 127 (fp32
+ * quotients, ties to even).
  * (Also quantises F.linear weights [N,K] per output channel, for qtts_pack_weight_int8.)
  * qtts_rmsnorm_int8: h = bf16(x + delta) is written to `sum` (which may be x or delta itself, with its stride); then
  * y = h / sqrt(mean(h^2) + eps) * w in fp32 (the mean too: it overflows where sum(h^2) does), not rounded in between,

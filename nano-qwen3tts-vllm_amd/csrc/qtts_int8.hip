@@ -2,7 +2,7 @@
 // RMSNorm), int8 weight packing, and the product of int8 rows with int8 weights on the int8 matrix instructions, plain
 // or with the SwiGLU epilogue.  An extension: the reference has bf16 only.
 //
-//   s_m = max(max_k |y_mk| / 127, 2^-126)      q_mk = rint(y_mk / s_m)            |q| <= 127
+//   s_m = max(max_k |y_mk| / 127, 2^-126)      q_mk = rint(y_mk / s_m)            |q| <= 127      (quotients in fp32)
 //   out_mn = bf16(xs_m * ws_n * sum_k q_mk w_nk [+ bias_n] [+ residual_mn])
 //
 // The sum is exact: |q w| <= 2^14, so int32 holds K <= 131071 of them whatever the order of the additions - the same
@@ -75,15 +75,53 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     v = max(v, (uint32_t)__shfl_xor((int)v, 16));
     return max(v, (uint32_t)__shfl_xor((int)v, 32));
 }
+// The largest magnitude of eight values and top; a NaN is larger than every number and stays.
+__device__ __forceinline__ float magnitude(float top, const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2)
+        top = __builtin_elementwise_maximum(__builtin_elementwise_maximum(__builtin_fabsf(v[j]), __builtin_fabsf(v[j + 1])), top);
+    return top;
+}
 // A row's scale from the bits of its largest magnitude.  NaN and infinity stay: the whole row then stands for NaN.
 __device__ __forceinline__ float i8_scale(uint32_t top) {
     const float s = __uint_as_float(top) / 127.0f;
     return s < I8_TINY ? I8_TINY : s;
 }
-// Eight columns from k0 on; inv 0 is a row that is not finite, and stands for zeros.
-__device__ __forceinline__ void store8_i8(int8_t *row, int k0, int K, float (&v)[8], float inv) {
+// a / b in fp32 with inv, the reciprocal of b rounded to nearest: the product is off by 1.5 units in the last place at most, and
+// the step of Markstein (IBM J. Res. Dev. 34, 1990) adds what is left of a, which a fused multiply-add gives (nearly) without
+// error.  For bf16 a and b = RN(bf16 / 127) >= 2^-100, all there is to quantising bf16 rows, it is the rounded quotient for every
+// pair of mantissas; otherwise it is that but for last bits decided by less than 2^-22 of a unit.  The product alone puts
+// 127 * (1/2), the half of a row's maximum, on the other side of 63.5 for some maxima.
+__device__ __forceinline__ float quotient(float a, float b, float inv) {
+    const float q = a * inv;
+    return __builtin_fmaf(__builtin_fmaf(-q, b, a), inv, q);
+}
+// What a row's values are divided by, with its reciprocal.  Rows that are not finite stand for zeros, and with a very small scale
+// up keeps what is left of a value a normal number: both are rare, the same in the whole wave, and behind one scalar branch.
+struct I8Div { float s, inv, up; bool rare; };
+__device__ __forceinline__ I8Div i8_div(uint32_t top, float s) {
+    I8Div d;
+    d.up = top >= 0x7f800000u ? 0.f : s < 0x1p-100f ? 0x1p100f : 1.0f;
+    d.s = d.up == 0.f ? 1.0f : s * d.up;
+    d.inv = 1.0f / d.s;
+    d.rare = __builtin_amdgcn_readfirstlane(__float_as_uint(d.up)) != 0x3f800000u;
+    return d;
+}
+// RMSNorm's h / root * w with rstd = 1 / root.  The root is infinite where the mean is: h / root is 0 then (NaN for an infinite h).
+__device__ __forceinline__ float i8_normed(float h, float root, float rstd, float w) { return quotient(h, root, rstd) * w; }
+__device__ __forceinline__ float i8_root(float mean_eps, float &rstd) {
+    const float root = sqrtf(mean_eps);
+    rstd = 1.0f / root;
+    return rstd == 0.f ? 0.f : root;
+}
+// Eight columns from k0 on.
+__device__ __forceinline__ void store8_i8(int8_t *row, int k0, int K, float (&v)[8], const I8Div &d) {
+    if (d.rare) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = inv != 0.f ? v[j] * inv : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = d.up != 0.f ? v[j] * d.up : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = quotient(v[j], d.s, d.inv);
     const uint2 p = make_uint2(pack4_i8(v[0], v[1], v[2], v[3]), pack4_i8(v[4], v[5], v[6], v[7]));
     if (k0 + 8 <= K) *reinterpret_cast<uint2 *>(row + k0) = p;
     else
@@ -138,7 +176,7 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
                 }
             }
         }
-        float rstd = 1.0f;
+        float root = 1.0f, rstd = 1.0f;
         if (NORM) {
             // Squares are added up per 512 columns (a chunk's 8, then the 64 lanes of a wave), then in the order of the columns:
             // the same sum, and the same row, whatever number of threads the launch chose.
@@ -164,21 +202,22 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 #pragma unroll
                 for (int c = 0; c < CH; ++c) ss += part[c];
             }
-            rstd = 1.0f / sqrtf(ss / (float)a.K + a.eps);
+            root = i8_root(ss / (float)a.K + a.eps, rstd);
         }
-        // the largest magnitude as an integer maximum over the numbers' bits: a NaN is above every number and stays
-        uint32_t top = 0;
+        // across lanes the maximum is one of integers, over the numbers' bits: a NaN is above every number and stays.  Columns
+        // behind the last are zeros (not where the root is 0 or NaN: then the row is not finite whatever they are)
+        float largest = 0.f;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
+            float v[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                float v = bf2f(h[c].h[j]);
-                if (NORM) v = v * rstd * bf2f(wv[c].h[j]);
-                // columns behind the last are zeros, also where rstd is not finite
-                if (NORM && !((c * T + t) * 8 + j < a.K)) v = 0.f;
-                top = max(top, __float_as_uint(v) & 0x7fffffffu);
+                v[j] = bf2f(h[c].h[j]);
+                if (NORM) v[j] = i8_normed(v[j], root, rstd, bf2f(wv[c].h[j]));
             }
+            largest = magnitude(largest, v);
         }
+        uint32_t top = __float_as_uint(largest) & 0x7fffffffu;
         top = wave_max(top);
         if (W > 1) {
             if ((t & 63) == 0) red_u[t >> 6] = top;
@@ -189,9 +228,8 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
             if (m + gridDim.x < (unsigned)a.M) __syncthreads();      // the next row writes red_* again
         }
         const float s = i8_scale(top);
-        const float inv = top < 0x7f800000u ? 1.0f / s : 0.f;
+        const I8Div by = i8_div(top, s);
         if (t == 0) a.scales[m] = s;
-        if (CH > 2) asm volatile("" : "+v"(rstd));        // the products again, rather than 8 CH of them kept in registers
         int8_t *qr = a.q + (size_t)m * a.ldq;
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
@@ -201,9 +239,9 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] = bf2f(h[c].h[j]);
-                if (NORM) v[j] = v[j] * rstd * bf2f(wv[c].h[j]);
+                if (NORM) v[j] = i8_normed(v[j], root, rstd, bf2f(wv[c].h[j]));
             }
-            store8_i8(qr, k0, a.K, v, inv);
+            store8_i8(qr, k0, a.K, v, by);
         }
     }
 }
@@ -218,7 +256,7 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
     const int t = threadIdx.x;
     for (int m = blockIdx.x; m < a.M; m += gridDim.x) {
         const bf16_t *xr = a.x + (size_t)m * a.ldx, *hr = xr;
-        float rstd = 1.0f;
+        float root = 1.0f, rstd = 1.0f;
         if (NORM) {
             float ss = 0.f;
             const bf16_t *dr = a.delta ? a.delta + (size_t)m * a.ldd : nullptr;
@@ -245,7 +283,7 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
             ss = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) ss += red_f[i];
-            rstd = 1.0f / sqrtf(ss / (float)a.K + a.eps);
+            root = i8_root(ss / (float)a.K + a.eps, rstd);
         }
         auto chunk = [&](int k0, float (&v)[8]) {
             Frag h, w;
@@ -254,32 +292,32 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 v[j] = bf2f(h.h[j]);
-                if (NORM) v[j] = k0 + j < a.K ? v[j] * rstd * bf2f(w.h[j]) : 0.f;
+                if (NORM) v[j] = i8_normed(v[j], root, rstd, bf2f(w.h[j]));
             }
         };
-        uint32_t top = 0;
+        float largest = 0.f;
 #pragma unroll 4
         for (int k0 = t * 8; k0 < a.K; k0 += 8192) {
             float v[8];
             chunk(k0, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
+            largest = magnitude(largest, v);
         }
-        top = wave_max(top);
+        uint32_t top = wave_max(__float_as_uint(largest) & 0x7fffffffu);
         if ((t & 63) == 0) red_u[t >> 6] = top;
         __syncthreads();
         top = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = max(top, red_u[i]);
         if (m + gridDim.x < (unsigned)a.M) __syncthreads();          // the next row writes red_* again
-        const float s = i8_scale(top), inv = top < 0x7f800000u ? 1.0f / s : 0.f;
+        const float s = i8_scale(top);
+        const I8Div by = i8_div(top, s);
         if (t == 0) a.scales[m] = s;
         int8_t *qr = a.q + (size_t)m * a.ldq;
 #pragma unroll 4
         for (int k0 = t * 8; k0 < a.K; k0 += 8192) {
             float v[8];
             chunk(k0, v);
-            store8_i8(qr, k0, a.K, v, inv);
+            store8_i8(qr, k0, a.K, v, by);
         }
     }
 }

@@ -293,7 +293,8 @@ def _int8_out(q, scales, M, K, x, what, dev):
 
 
 def quantize_int8(x, out=None, scales=None):
-    """bf16 rows [M, K] -> (int8 [M, K], fp32 scale per row): q = rint(x / scale), scale = max(max|x| / 127, 2^-126)."""
+    """bf16 rows [M, K] -> (int8 [M, K], fp32 scale per row): q = rint(x / scale), scale = max(max|x| / 127, 2^-126),
+    quotients in fp32."""
     dev = _device_of(x, "quantize_int8: x")
     M, K, ldx = _rows_of(x, torch.bfloat16, "quantize_int8: x", dev)
     out, ldq, scales = _int8_out(out, scales, M, K, x, "quantize_int8", dev)
