@@ -234,8 +234,12 @@ def _device_of(t, what):
     return dev
 
 
+INT_MAX = 0x7fffffff
+
+
 def _rows_of(t, dtype, what, dev, rows=None, cols=None):
-    """(rows, columns, row stride) of a matrix with contiguous columns."""
+    """(rows, columns, row stride) of a matrix with contiguous columns.  ctypes keeps the low 32 bits of a larger number, so the
+    library's own checks would see another, valid one: it is refused here.  A single row has no stride of its own."""
     if t.get_device() != dev or t.dtype is not dtype or t.dim() != 2:
         raise QttsError(f"{what}: need [rows, columns] of {dtype} on device {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
     M, K = t.shape
@@ -244,7 +248,11 @@ def _rows_of(t, dtype, what, dev, rows=None, cols=None):
         raise QttsError(f"{what}: need contiguous columns, got strides {t.stride()}")
     if rows is not None and (M != rows or K != cols):
         raise QttsError(f"{what}: shape {(M, K)}, need {(rows, cols)}")
-    return M, K, ld if M > 1 or ld > K else K
+    if M == 1:
+        ld = K
+    if M > INT_MAX or K > INT_MAX or ld > INT_MAX:
+        raise QttsError(f"{what}: shape {(M, K)}, row stride {ld}: need numbers below 2^31")
+    return M, K, ld
 
 
 def _vector_of(t, dtype, what, dev, n):
@@ -272,7 +280,7 @@ def _int8_rows_of(t, what, dev, rows=None, cols=None):
     M, K, ld = _rows_of(t, torch.int8, what, dev, rows, cols)
     if K % 16:
         pad = (K + 15) // 16 * 16
-        if M == 1 and ld < pad:
+        if M == 1:
             ld = pad
         if t.storage_offset() + (M - 1) * ld + pad > t.untyped_storage().nbytes():
             raise QttsError(f"{what}: {K} columns, but a row needs {pad} readable bytes (int8_rows allocates them)")

@@ -75,3 +75,17 @@ def test_normed_rows_whose_mean_overflows(hip):
     x[2, 5] = float("inf")
     q, s = hip.rmsnorm_int8(x.to(DEV), torch.ones(600, dtype=torch.bfloat16, device=DEV), 1e-6)
     assert not q.any() and s[:2].tolist() == [TINY, TINY] and bool(torch.isnan(s[2]))
+
+
+@pytest.mark.parametrize("K", [992, 990])
+def test_a_single_row_of_a_wider_buffer(hip, K):
+    """Its stride means nothing and may be anything: also one that rows of int8 values could not have."""
+    g = torch.Generator(device=DEV).manual_seed(K)
+    x = torch.randn(3, 1000, generator=g, device=DEV).bfloat16()[:1, :K]
+    qbuf = torch.full((3, 1000), 99, dtype=torch.int8, device=DEV)
+    q, s = hip.quantize_int8(x, out=qbuf[:1, :K])
+    want, want_s = hip.quantize_int8(x.contiguous())
+    assert torch.equal(q, want) and torch.equal(s, want_s) and torch.all(qbuf[:1, K:] == 99) and torch.all(qbuf[1:] == 99)
+    w, ws = torch.randint(-128, 128, (40, K), generator=g, device=DEV, dtype=torch.int8), torch.ones(40, device=DEV)
+    p = hip.pack_weight_int8(w)
+    assert torch.equal(hip.linear_int8(q, s, p, ws, 40), hip.linear_int8(want, s, p, ws, 40))

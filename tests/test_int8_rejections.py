@@ -98,3 +98,26 @@ def test_wrappers_refuse_what_is_not_on_the_device():
                  lambda: hip.linear_swiglu_int8(q, v, p, torch.ones(8), torch.ones(8), 8)):
         with pytest.raises(hip.QttsError, match="on cpu"):
             call()
+
+
+def test_wrappers_refuse_numbers_beyond_an_int():
+    """ctypes hands on the low 32 bits: 2^32 + 64 would arrive as 64.  (meta tensors: shapes and strides without memory)"""
+    def rows(M, K, ld, dtype=torch.bfloat16):
+        return torch.empty_strided((M, K), (ld, 1), dtype=dtype, device="meta")
+
+    for M, K, ld in ((2, 64, 2 ** 32 + 64), (2, 64, 2 ** 31), (2 ** 32 + 4, 64, 64), (2 ** 31, 1, 1), (3, 2 ** 32 + 64, 2 ** 32 + 64)):
+        for call, dtype in ((hip._rows_of, torch.bfloat16), (hip._rows_of, torch.int8)):
+            with pytest.raises(hip.QttsError, match="below 2"):
+                call(rows(M, K, ld, dtype), dtype, "x", -1)
+        with pytest.raises(hip.QttsError, match="below 2"):
+            hip._int8_rows_of(rows(M, K, ld, torch.int8), "x", -1)
+    assert hip._rows_of(rows(2, 64, 2 ** 31 - 1), torch.bfloat16, "x", -1) == (2, 64, 2 ** 31 - 1)
+
+
+def test_a_single_row_has_no_stride_of_its_own():
+    wide = torch.zeros(3, 1000, dtype=torch.int8)
+    assert hip._int8_rows_of(wide[:1, :992], "x", -1) == (1, 992, 992)
+    assert hip._int8_rows_of(wide[:1, :990], "x", -1) == (1, 990, 992)
+    assert hip._rows_of(torch.empty_strided((1, 64), (2 ** 40, 1), dtype=torch.bfloat16, device="meta"), torch.bfloat16, "x", -1) == (1, 64, 64)
+    with pytest.raises(hip.QttsError, match="readable bytes"):
+        hip._int8_rows_of(torch.zeros(1, 60, dtype=torch.int8), "x", -1)
