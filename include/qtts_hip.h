@@ -137,6 +137,11 @@ int qtts_linear_swiglu_int8(const void *x, int ldx, const float *x_scales, const
                             const float *gate_scales, const float *up_scales, void *out, int ldo, int M, int I, int K,
                             qtts_stream_t stream);
 
+/* The form that a product of this shape takes: 0-4 K over the waves of a workgroup, 5 half a packed tile a workgroup, 6-10 tiles
+ * through LDS (64x64, 128x128 one k-step a stage, 128x128, 128x256, 256x256); -1 for a shape that is refused.  Every form gives
+ * the same bits: this is for tests and measurements, and runs on the host alone. */
+int qtts_linear_int8_form(int M, int N, int K, int swiglu);
+
 /* out[M,I] = silu(x@Wg^T) * (x@Wu^T) with the reference's two roundings
  * (P/models/qwen3_tts_share.py:131-135, P/layers/activation.py:11-13);
  * optional fused RMSNorm of x as above. */

@@ -974,6 +974,12 @@ static int choose_int8_form(int M, int columns, int K) {
     return best;
 }
 
+extern "C" int qtts_linear_int8_form(int M, int N, int K, int swiglu) {
+    QCHECK(M > 0 && M <= I8_MAX_ROWS && N > 0 && N <= I8_MAX_N && K > 0 && K <= I8_MAX_K, "linear_int8_form: bad shape M=%d N=%d K=%d (M <= %d, N <= %d, K <= %d)",
+           M, N, K, I8_MAX_ROWS, I8_MAX_N, I8_MAX_K);
+    return choose_int8_form(M, 16 * ceil_div(N, swiglu ? 8 : 16), K);
+}
+
 template <bool SWIGLU>
 static void launch_int8_form(const LinI8Args &a, int tiles, int form, hipStream_t s) {
 #define QTTS_TILE_I8(BM, BN, WM, WN, KS, ST, ALT, PER_CU) do { const int mt = ceil_div(a.M, BM), nt = ceil_div(tiles, BN / 16); \

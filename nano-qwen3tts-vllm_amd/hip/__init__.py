@@ -53,6 +53,7 @@ _SIGS = {
     "qtts_pack_gate_up_int8": (_i, [_p, _p, _i, _p, _i, _i, _p]),
     "qtts_linear_int8": (_i, [_p, _i, _p, _p, _p, _p, _p, _i, _p, _i, _i, _i, _i, _p]),
     "qtts_linear_swiglu_int8": (_i, [_p, _i, _p, _p, _p, _p, _p, _i, _i, _i, _i, _p]),
+    "qtts_linear_int8_form": (_i, [_i, _i, _i, _i]),
     "qtts_linear_swiglu": (_i, [_p, _i, _p, _p, _f, _p, _i, _i, _i, _i, _p]),
     "qtts_rmsnorm": (_i, [_p, _i, _p, _f, _p, _i, _i, _i, _p]),
     "qtts_qknorm_rope_store": (_i, [_p, _i, _p, _p, _f, _p, _p, _i, _p, _p, _p, _p, _i, _i, _i, _p]),

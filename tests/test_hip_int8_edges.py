@@ -3,6 +3,8 @@ integers, results next to the end of fp32's range, and the tiled forms of the pr
 import pytest
 import torch
 
+from test_hip_int8 import check_product, exact_swiglu, product_case, swiglu_case
+
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
 TINY = 2.0 ** -126
@@ -89,3 +91,80 @@ def test_a_single_row_of_a_wider_buffer(hip, K):
     w, ws = torch.randint(-128, 128, (40, K), generator=g, device=DEV, dtype=torch.int8), torch.ones(40, device=DEV)
     p = hip.pack_weight_int8(w)
     assert torch.equal(hip.linear_int8(q, s, p, ws, 40), hip.linear_int8(want, s, p, ws, 40))
+
+
+# ---------------------------------------------------------------- the product in every form
+# (form, M, N, K): forms 0-5 split K over waves, 6-10 are the tiles.  For each tile: at most a tile a workgroup and several, two
+# k-steps (fewer than the stages that are requested ahead) and many; nothing is a multiple of anything.  Form 8 takes
+# shapes with at most 256 tiles only, which is a tile a workgroup.  A row or column more or less may change the form, so the
+# form is asserted (also on the host, in the tests that need no device).
+LINEAR_FORMS = [
+    (0, 108, 356, 1180), (0, 360, 69, 1093), (1, 11, 1319, 2308), (1, 185, 85, 2390), (2, 230, 46, 172), (2, 9, 4535, 179),
+    (3, 353, 453, 355), (4, 693, 439, 129), (5, 12, 82, 2651), (5, 25, 358, 365),
+    (6, 1111, 872, 980), (6, 2898, 944, 4), (6, 8446, 203, 144), (6, 323, 5781, 657),
+    (7, 2600, 2558, 156), (7, 1351, 5867, 3), (7, 2615, 3179, 134), (7, 1924, 4447, 656),
+    (8, 1549, 1507, 660), (8, 2916, 1353, 176), (8, 1301, 2713, 3),
+    (9, 3151, 1330, 660), (9, 4880, 1495, 130), (9, 4964, 3222, 742),
+    (10, 2070, 5994, 663), (10, 5946, 2321, 258), (10, 6514, 4830, 587), (10, 5625, 5573, 642),
+]
+SWIGLU_FORMS = [
+    (0, 148, 135, 1562), (1, 11, 1091, 1501), (2, 593, 26, 243), (3, 100, 667, 222), (4, 196, 830, 310), (5, 23, 79, 230),
+    (6, 303, 929, 1660), (6, 664, 1585, 267), (6, 6510, 421, 2),
+    (7, 4916, 779, 648), (7, 2647, 3729, 155), (7, 3500, 4635, 2),
+    (8, 2692, 419, 654), (8, 579, 2509, 134), (8, 2570, 611, 3),
+    (9, 2900, 721, 643), (9, 1477, 2649, 129), (9, 2595, 2995, 724),
+    (10, 4465, 1391, 654), (10, 1344, 5046, 265), (10, 8846, 1749, 558),
+]
+
+
+def inside(M, N, wider, offset):
+    """A view [M, N] with a row stride of N + wider, `offset` elements into a buffer of sevens, and a check that the rest of
+    the buffer still holds them."""
+    buf = torch.full((offset + M * (N + wider) + 9,), 7.0, dtype=torch.bfloat16, device=DEV)
+    view = buf.as_strided((M, N), (N + wider, 1), offset)
+
+    def rest_is_untouched():
+        inside = torch.zeros_like(buf, dtype=torch.bool)
+        inside.as_strided((M, N), (N + wider, 1), offset).fill_(True)
+        return bool(((buf == 7.0) | inside).all())
+
+    return view, rest_is_untouched
+
+
+@pytest.mark.parametrize("form,M,N,K", LINEAR_FORMS)
+def test_linear_in_every_form(hip, form, M, N, K):
+    """Dense, and with bias and residual into the residual's own place inside a wider buffer at odd alignments: float64, and the
+    same bits as into a buffer of its own."""
+    assert hip.lib.qtts_linear_int8_form(M, N, K, 0) == form
+    x, xs, w, ws, b, r = product_case(hip, M, N, K, True, True, seed=1)
+    p = hip.pack_weight_int8(w)
+    check_product(hip.linear_int8(x, xs, p, ws, N), x, xs, w, ws)
+    got = hip.linear_int8(x, xs, p, ws, N, bias=b, residual=r)
+    check_product(got, x, xs, w, ws, b, r)
+    wide = torch.full((M, (K + 15) // 16 * 16 + 48), -1, dtype=torch.int8, device=DEV)[:, 16:16 + K]
+    wide.copy_(x)
+    assert torch.equal(hip.linear_int8(wide, xs, p, ws, N, bias=b, residual=r), got)
+    for wider, offset in ((5, 3), (8, 8)):
+        view, rest_is_untouched = inside(M, N, wider, offset)
+        view.copy_(r)
+        assert hip.linear_int8(x, xs, p, ws, N, bias=b, residual=view, out=view) is view
+        assert torch.equal(view, got) and rest_is_untouched()
+        other, rest_is_untouched = inside(M, N, wider + 4, offset + 1)
+        view.copy_(r)
+        hip.linear_int8(x, xs, p, ws, N, bias=b, residual=view, out=other)
+        assert torch.equal(other, got) and rest_is_untouched() and torch.equal(view, r)
+
+
+@pytest.mark.parametrize("form,M,I,K", SWIGLU_FORMS)
+def test_swiglu_in_every_form(hip, form, M, I, K):
+    assert hip.lib.qtts_linear_int8_form(M, I, K, 1) == form
+    x, xs, gate, gs, up, us = swiglu_case(hip, M, I, K)
+    p = hip.pack_gate_up_int8(gate, up)
+    got = hip.linear_swiglu_int8(x, xs, p, gs, us, I)
+    g, u, want = exact_swiglu(x, xs, gate, gs, up, us)
+    off = (got.double() - want).abs() - ((2.0 ** -8 + (g.abs() + 2) * 2.0 ** -20) * want.abs() + 2.0 ** -118 * (g * u).abs())
+    assert float(off.max()) <= 0, float(off.max())
+    for wider, offset in ((5, 3), (8, 8)):
+        view, rest_is_untouched = inside(M, I, wider, offset)
+        hip.linear_swiglu_int8(x, xs, p, gs, us, I, out=view)
+        assert torch.equal(view, got) and rest_is_untouched()

@@ -121,3 +121,14 @@ def test_a_single_row_has_no_stride_of_its_own():
     assert hip._rows_of(torch.empty_strided((1, 64), (2 ** 40, 1), dtype=torch.bfloat16, device="meta"), torch.bfloat16, "x", -1) == (1, 64, 64)
     with pytest.raises(hip.QttsError, match="readable bytes"):
         hip._int8_rows_of(torch.zeros(1, 60, dtype=torch.int8), "x", -1)
+
+
+def test_the_form_of_a_product():
+    """A host-only query.  The device tests cover every form: a change of the choice must not take one out of them."""
+    import test_hip_int8_edges as edges
+    for swiglu, cases in enumerate((edges.LINEAR_FORMS, edges.SWIGLU_FORMS)):
+        for form, M, N, K in cases:
+            assert L.qtts_linear_int8_form(M, N, K, swiglu) == form, (M, N, K, swiglu)
+        assert {case[0] for case in cases} == set(range(11))
+    for M, N, K in ((0, 1, 1), (1, 0, 1), (1, 1, 0), (1, 1, 131072), (1, 0x4000000, 1), (0x7f800001, 1, 1)):
+        assert L.qtts_linear_int8_form(M, N, K, 0) == -1 and L.qtts_linear_int8_form(M, N, K, 1) == -1
