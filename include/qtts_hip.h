@@ -103,7 +103,8 @@ int qtts_linear_swiglu_fp8(const void *x, int ldx, const void *w_gate_up_fp8_pac
 
 /* ---- 8-bit integers (W8A8): an extension, the reference has bf16 only.  Activation rows and weight rows are int8 with one
  * fp32 scale each, a row standing for q * scale.  A product's integer sum is exact (int32, K <= 131071); what follows it is
- * fp32 with ONE rounding, to bf16, at the store.  int8 activations are [M, ld] with ld % 16 == 0, 16-byte aligned: the bytes
+ * fp32 with ONE rounding, to bf16, at the store, and passes fp32's range only where sum * scales does (infinite then; SwiGLU of
+ * a gate of minus infinity is NaN).  int8 activations are [M, ld] with ld % 16 == 0, 16-byte aligned: the bytes
  * K .. round_up(K, 16) of every row (the last one included) must be readable, whatever they hold, and are never written.
  * M, N, I >= 1 and K, H >= 1 are free of multiples, bf16 rows of strides and alignment; a row's result does not depend on
  * the number of rows, nor on the rows beside it.  M <= 2139095040, N and I <= 67108863.  A row that holds a NaN or an

@@ -9,6 +9,7 @@
 // result for every tile shape and every split of K, which is why the launch is free to choose both by speed alone.
 // Everything after the sum is fp32 with one rounding to bf16 at the store.
 #include "qtts_common.h"
+#include <type_traits>
 
 typedef int int4_t __attribute__((ext_vector_type(4)));
 
@@ -436,17 +437,24 @@ struct LinI8Args {
     int M, N, K, ksteps;           // N: output columns; ksteps: of a packed tile
 };
 
-// What follows a sum, in the same operations in every kernel: a row's result does not depend on the form it came from.
-__device__ __forceinline__ float i8_scaled(int acc, float xs, float ws, float bias) { return __builtin_fmaf((float)acc * xs, ws, bias); }
-__device__ __forceinline__ float i8_swiglu(int g, int u, float xs, float gs, float us) {
-    return silu_f((float)g * xs * gs) * ((float)u * xs * us);
+// What follows a sum, in the same operations in every kernel: a row's result does not depend on the form it came from.  A sum
+// is below 2^31, so times a row scale of 2^96 or more it might pass fp32's range although the result does not: the channel's
+// scale comes first then, and passes the range only with the result.  (Not for NaN, which stays in either order.)
+struct I8Scale { float row; bool later; };
+__device__ __forceinline__ I8Scale i8_row_scale(float xs) { return {xs, __builtin_fabsf(xs) >= 0x1p96f}; }
+__device__ __forceinline__ float i8_scaled(int acc, I8Scale x, float ws, float bias) {
+    return __builtin_fmaf((float)acc * (x.later ? ws : x.row), x.later ? x.row : ws, bias);
+}
+__device__ __forceinline__ float i8_swiglu(int g, int u, I8Scale x, float gs, float us) {
+    const float gate = (float)g * (x.later ? gs : x.row) * (x.later ? x.row : gs);
+    return silu_f(gate) * ((float)u * (x.later ? us : x.row) * (x.later ? x.row : us));
 }
 
 // One 16 x 16 tile of sums, this lane's four of them: weight rows 4 * (lane / 16) .. +3 of `tile`, activation row m.
 template <bool SWIGLU>
 __device__ __forceinline__ void i8_store(const LinI8Args &a, int4_t acc, int tile, int m, int lane) {
     if (m >= a.M) return;
-    const float xs = a.xs[m];
+    const I8Scale xs = i8_row_scale(a.xs[m]);
     bf16_t *o = a.out + (size_t)m * a.ldo;
     if (SWIGLU) {
         const int n = 8 * tile + 2 * (lane >> 4);
@@ -838,7 +846,7 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
         // every pass.  The 16-byte chunk c of row q lies at place c ^ q (modulo the chunks of a row, 16 at most).
         int4_t *mine = reinterpret_cast<int4_t *>(lds + (OVER ? ST - 1 : ST) * STAGE) + wave * HT * 64 * TN;
         const int lrow = lane / LPR, c = lane % LPR;
-        auto outputs = [&](int pass, float xs, float (&y)[OUT]) {
+        auto outputs = [&](int pass, I8Scale xs, float (&y)[OUT]) {
             const int4_t *v = mine + (pass * RPP + lrow) * (TN * 4);
             const int turn = (lrow & CMASK) ^ ((pass * RPP) & CMASK);
             if (SWIGLU) {
@@ -863,60 +871,70 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
         const size_t ostep = (size_t)RPP * a.ldo;
         // every pass stores something: the rows are there, and the wave's first columns
         loose = row0 + TM * 16 <= a.M && nw < whole ? ST - 1 : 0;
+        // Rows whose scale comes last (i8_row_scale) are rare: the two selects an output that they need, 3-4 % of the time (SwiGLU
+        // 8192 x 6144 x 2048 193 -> 200 us), are in a copy of the epilogue for waves that have such a row.
+        auto epilogue = [&](auto huge_rows) {
+            auto scale = [](float xs) { return decltype(huge_rows)::value ? i8_row_scale(xs) : I8Scale{xs, false}; };
 #pragma unroll
-        for (int h = 0; h < TM; h += HT) {
+            for (int h = 0; h < TM; h += HT) {
 #pragma unroll
-            for (int i = 0; i < HT; ++i)
+                for (int i = 0; i < HT; ++i)
 #pragma unroll
-                for (int j = 0; j < TN; ++j) mine[(16 * i + r) * (TN * 4) + ((4 * j + g) ^ (r & CMASK))] = acc[h + i][j];
-            __builtin_amdgcn_wave_barrier();
+                    for (int j = 0; j < TN; ++j) mine[(16 * i + r) * (TN * 4) + ((4 * j + g) ^ (r & CMASK))] = acc[h + i][j];
+                __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int p = 0; p < NP; ++p) {
-                float y[OUT];
-                outputs(p, row_scale(h * 16 + p * RPP), y);
-                if (add) {
-                    const int pass = h / HT * NP + p;
+                for (int p = 0; p < NP; ++p) {
+                    float y[OUT];
+                    outputs(p, scale(row_scale(h * 16 + p * RPP)), y);
+                    if (add) {
+                        const int pass = h / HT * NP + p;
 #pragma unroll
-                    for (int j = 0; j < OUT; j += 2) {
-                        float lo, hi;
-                        unpack2(rf[pass % RB][j / 2], lo, hi);
-                        y[j] += lo;
-                        y[j + 1] += hi;
+                        for (int j = 0; j < OUT; j += 2) {
+                            float lo, hi;
+                            unpack2(rf[pass % RB][j / 2], lo, hi);
+                            y[j] += lo;
+                            y[j + 1] += hi;
+                        }
+                        if (pass + RB < PASSES) rf[pass % RB] = residual(pass + RB);
                     }
-                    if (pass + RB < PASSES) rf[pass % RB] = residual(pass + RB);
-                }
-                uint32_t packed[OUT / 2];
+                    uint32_t packed[OUT / 2];
 #pragma unroll
-                for (int j = 0; j < OUT; j += 2) packed[j / 2] = pack2v(float2_t{y[j], y[j + 1]});
-                if (h * 16 + p * RPP < have) {
-                    // nothing of this launch reads the output again: kept out of the way of the rows and weights in L2 (2-4 %)
-                    if constexpr (OUT == 8)
-                        __builtin_nontemporal_store(u32x4_t{packed[0], packed[1], packed[2], packed[3]}, reinterpret_cast<u32x4_any *>(op));
-                    else __builtin_nontemporal_store(u32x2_t{packed[0], packed[1]}, reinterpret_cast<u32x2_any *>(op));
-                }
-                op += ostep;
-            }
-            if (rest) {                                            // neighbouring lanes neighbouring columns, 64 / OUT rows at a time
-                const int tc = lane % OUT, n = min(whole + tc, a.N - 1), col = n - nw;
-                const int pc = SWIGLU ? (col >> 1) * 4 + (col & 1) : col;                  // packed column of the sum (of the gate's)
-                const int *flat = reinterpret_cast<const int *>(mine);
-                const float s0 = a.ws[n], s1 = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
-#pragma unroll
-                for (int e = 0; e < 16 * HT * OUT / 64; ++e) {
-                    const int row = e * (64 / OUT) + lane / OUT, m = min(row0 + h * 16 + row, a.M - 1);
-                    const int at = (row * (TN * 4) + ((pc >> 2) ^ (row & CMASK))) * 4 + (pc & 3);
-                    const float xs = __shfl(now.xs[h >> 2], (h & 3) * 16 + row);
-                    float y;
-                    if (SWIGLU) y = i8_swiglu(flat[at], flat[at + 2], xs, s0, s1);
-                    else {
-                        y = i8_scaled(flat[at], xs, s0, s1);
-                        if (a.res) y += bf2f(a.res[(size_t)m * a.ldr + n]);
+                    for (int j = 0; j < OUT; j += 2) packed[j / 2] = pack2v(float2_t{y[j], y[j + 1]});
+                    if (h * 16 + p * RPP < have) {
+                        // nothing of this launch reads the output again: kept out of the way of the rows and weights in L2 (2-4 %)
+                        if constexpr (OUT == 8)
+                            __builtin_nontemporal_store(u32x4_t{packed[0], packed[1], packed[2], packed[3]}, reinterpret_cast<u32x4_any *>(op));
+                        else __builtin_nontemporal_store(u32x2_t{packed[0], packed[1]}, reinterpret_cast<u32x2_any *>(op));
                     }
-                    if (row0 + h * 16 + row < a.M && whole + tc < a.N) a.out[(size_t)m * a.ldo + n] = f2bf(y);
+                    op += ostep;
                 }
+                if (rest) {                                            // neighbouring lanes neighbouring columns, 64 / OUT rows at a time
+                    const int tc = lane % OUT, n = min(whole + tc, a.N - 1), col = n - nw;
+                    const int pc = SWIGLU ? (col >> 1) * 4 + (col & 1) : col;                  // packed column of the sum (of the gate's)
+                    const int *flat = reinterpret_cast<const int *>(mine);
+                    const float s0 = a.ws[n], s1 = SWIGLU ? a.us[n] : a.bias ? bf2f(a.bias[n]) : 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16 * HT * OUT / 64; ++e) {
+                        const int row = e * (64 / OUT) + lane / OUT, m = min(row0 + h * 16 + row, a.M - 1);
+                        const int at = (row * (TN * 4) + ((pc >> 2) ^ (row & CMASK))) * 4 + (pc & 3);
+                        const I8Scale xs = scale(__shfl(now.xs[h >> 2], (h & 3) * 16 + row));
+                        float y;
+                        if (SWIGLU) y = i8_swiglu(flat[at], flat[at + 2], xs, s0, s1);
+                        else {
+                            y = i8_scaled(flat[at], xs, s0, s1);
+                            if (a.res) y += bf2f(a.res[(size_t)m * a.ldr + n]);
+                        }
+                        if (row0 + h * 16 + row < a.M && whole + tc < a.N) a.out[(size_t)m * a.ldo + n] = f2bf(y);
+                    }
+                }
+                __builtin_amdgcn_wave_barrier();
             }
-            __builtin_amdgcn_wave_barrier();
-        }
+        };
+        bool huge = false;
+#pragma unroll
+        for (int j = 0; j < XW; ++j) huge |= i8_row_scale(now.xs[j]).later;
+        if (__builtin_expect(__any(huge), 0)) epilogue(std::true_type{});
+        else epilogue(std::false_type{});
     }
 }
 

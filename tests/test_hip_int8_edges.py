@@ -168,3 +168,47 @@ def test_swiglu_in_every_form(hip, form, M, I, K):
         view, rest_is_untouched = inside(M, I, wider, offset)
         hip.linear_swiglu_int8(x, xs, p, gs, us, I, out=view)
         assert torch.equal(view, got) and rest_is_untouched()
+
+
+# ---------------------------------------------------------------- results next to the end of fp32's range
+def one_of_each_form(cases):
+    return [next(c for c in cases if c[0] == form) for form in range(11)]
+
+
+def huge_rows(x, xs):
+    """Every fifth row with the scale of a row at bf16's maximum or near it, a row of NaN, and a row of infinity as the row
+    operators leave it."""
+    xs[::5] = 2.6e36 * (0.5 + 0.5 * torch.rand_like(xs[::5]))
+    xs[1], xs[2] = float("nan"), float("inf")
+    x[1], x[2] = 0, 0
+    fine = torch.ones_like(xs, dtype=torch.bool)
+    fine[1:3] = False
+    return fine
+
+
+@pytest.mark.parametrize("form,M,N,K", one_of_each_form(LINEAR_FORMS))
+def test_linear_of_huge_rows(hip, form, M, N, K):
+    """Sum times row scale passes fp32's range, the result does not (|sum| <= 2^14 K < 2^26, channel scales of at most 2^-24)."""
+    x, xs, w, ws, b, r = product_case(hip, M, N, K, True, True, seed=2)
+    fine = huge_rows(x, xs)
+    ws = (0.1 + 0.9 * torch.rand_like(ws)) * 2.0 ** -24
+    got = hip.linear_int8(x, xs, hip.pack_weight_int8(w), ws, N, bias=b, residual=r)
+    assert torch.isnan(got[~fine]).all()
+    check_product(got[fine], x[fine], xs[fine], w, ws, b, r[fine])
+    assert float(got[fine].abs().max()) > 2.0 ** 100
+
+
+@pytest.mark.parametrize("form,M,I,K", one_of_each_form(SWIGLU_FORMS))
+def test_swiglu_of_huge_rows(hip, form, M, I, K):
+    """The bound of the other sizes; for positive gates silu's relative slope stays below 1.3, so that |g| does not enter it.  The
+    rows that are not huge have gates and products of 1e-25 each here, whose product is below the smallest normal number: half a
+    step of a denormal bf16 number is 2^-134, of an fp32 one 2^-150, together below 2^-133."""
+    x, xs, gate, gs, up, us = swiglu_case(hip, M, I, K)
+    fine = huge_rows(x, xs)
+    gs, us = (t / t.max() * 2.0 ** -100 for t in (gs, us))
+    got = hip.linear_swiglu_int8(x, xs, hip.pack_gate_up_int8(gate, up), gs, us, I).double()
+    assert torch.isnan(got[~fine]).all()
+    g, u, want = (t[fine] for t in exact_swiglu(x, xs, gate, gs, up, us))
+    off = (got[fine] - want).abs() - ((2.0 ** -8 + (3 + (-g).clamp_min(0)) * 2.0 ** -20) * want.abs() + 2.0 ** -118 * (g * u).abs() + 2.0 ** -133)
+    assert float(off.max()) <= 0, float(off.max())
+    assert float(got[fine].abs().max()) > 2.0 ** 40
