@@ -28,7 +28,7 @@ def needs_build(out=OUT):
     if not os.path.exists(out):
         return True
     t = os.path.getmtime(out)
-    deps = SRC + [os.path.join(ROOT, "include", "qtts_hip.h"), os.path.join(HERE, "qtts_common.h")]
+    deps = SRC + [os.path.abspath(__file__), os.path.join(ROOT, "include", "qtts_hip.h"), os.path.join(HERE, "qtts_common.h")]
     if out == OUT_TUNING:
         deps += [os.path.join(HERE, "qtts_tuning.h")]
     return any(os.path.getmtime(d) > t for d in deps)

@@ -136,3 +136,22 @@ def test_single_caller_guard_is_reentrant_for_one_thread_and_refuses_a_second():
     t.start()
     t.join()
     assert seen[2] == "entered"
+
+
+def test_a_change_of_the_build_script_builds_again(monkeypatch):
+    """The compiler flags stand in build.py: libraries older than it, the measurement build too, are not up to date."""
+    import importlib.util
+    path = os.path.join(ROOT, "nano-qwen3tts-vllm_amd", "csrc", "build.py")
+    spec = importlib.util.spec_from_file_location("qtts_build_check", path)
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    changed = {}
+    monkeypatch.setattr(build.os.path, "exists", lambda p: True)
+    monkeypatch.setattr(build.os.path, "getmtime", lambda p: 100.0 if p.endswith(".so") else changed.get(os.path.basename(p), 50.0))
+    for out in (build.OUT, build.OUT_TUNING):
+        changed.clear()
+        assert not build.needs_build(out)
+        for name in ("build.py", "qtts_int8.hip", "qtts_hip.h", "qtts_common.h"):
+            changed.clear()
+            changed[name] = 200.0
+            assert build.needs_build(out), name
