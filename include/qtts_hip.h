@@ -109,6 +109,7 @@ int qtts_linear_swiglu_fp8(const void *x, int ldx, const void *w_gate_up_fp8_pac
  * M, N, I >= 1 and K, H >= 1 are free of multiples, bf16 rows of strides and alignment; a row's result does not depend on
  * the number of rows, nor on the rows beside it.  M <= 2139095040, N and I <= 67108863.  A row that holds a NaN or an
  * infinity gets a scale that is NaN or infinite and q = 0: everything computed from that row is NaN, no other row is touched.
+ * What a call writes overlaps what it reads only where that is said below.
  *
  * qtts_quantize_int8: scales[m] = max(max|x[m]| / 127, 2^-126), q[m] = rint(x[m] / scales[m]), |q| <= 127 (fp32
  * quotients, ties to even).

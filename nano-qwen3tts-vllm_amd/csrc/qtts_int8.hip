@@ -132,9 +132,9 @@ __device__ __forceinline__ void store8_i8(int8_t *row, int k0, int K, float (&v)
 // A row per T = 64 * W threads, R rows a workgroup; thread t of a row holds the 8-column chunks t, t + T, ... (CH of them) as
 // bf16 across both reductions, so x, delta and the weights are read once and nothing is read back.  All of a thread's
 // requests go out before its first store: sum may be x or delta, and a load behind a store that may alias waits for it.
-// Few rows are bound by the chain request - sum of squares - maximum - store (8 rows of 2048 with delta 3.6 us, an empty launch
-// 2.3), many by memory: 16384 x 2048 with delta 44.3 us, 5.3 TB/s of the 4.9-5.4 a large copy reaches; 8192 x 6144 quantised
-// alone 24.3 us, 6.2 TB/s (part of what it reads is in the caches still).
+// Few rows are bound by the chain request - sum of squares - maximum - store (8 rows of 2048 with delta 3.2 us, an empty launch
+// 2.3), many by memory and, without delta, by arithmetic too: 16384 x 2048 with delta 39.5 us, 5.9 TB/s (a large copy reaches
+// 4.9-5.4), without 24.3 us, 4.1 TB/s (23.0 with products in the quotients' place); 8192 x 6144 quantised alone 26.7 us, 5.7 TB/s.
 template <int W, int R, int CH, bool NORM>
 __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
     constexpr int T = W * 64;
@@ -249,7 +249,7 @@ __global__ __launch_bounds__(W * R * 64) void rows_int8_kernel(RowsI8Args a) {
 
 // Rows too long for registers: three walks over the row, the second and third of them out of L2 - h is read back from where
 // the first walk wrote it (sum), or from x.  Bound by those walks' latencies, a workgroup a row: 300 rows of 40000 columns 12 us
-// quantised, 36 us with norm and delta (the form above, whose chunks such rows push out of the registers: 94 us).
+// quantised, 32 us with norm and delta (floor 9 and 18 with the launch; the form above, whose chunks such rows push out of the registers: 94 us).
 template <bool NORM>
 __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
     __shared__ float red_f[16];
@@ -324,9 +324,9 @@ __global__ __launch_bounds__(1024) void rows_int8_long_kernel(RowsI8Args a) {
 }
 
 // Threads per row.  Few rows: as many as leave a chunk or two each, the launch is a chain of latencies (8 rows of 6144, with
-// delta: 4.2 us with 512 threads, 4.7 with 256, 5.0 with 64).  Many rows: fewer waves a row and more rows in flight
-// (8192 rows of 6144 with delta: 65 us, 5.4 TB/s, with 256 threads, 72 with 512; 16384 of 2048: 44.5 us with 128, 46.1 with 256,
-// 61 with 512; 16384 of 256: 12 us with a wave, 26 with 256 threads).
+// delta: 3.9 us with 512 threads, 4.5 with 256).  Many rows: fewer waves a row and more rows in flight (8192 rows of 6144 with
+// delta: 67 us, 5.3 TB/s, with 256 threads, 72 with 512; 16384 of 2048: 39.4 us with 128, 41.8 with 256, 56 with 512; 16384 of
+// 256: 9.9 us with a wave, 14 with 128 threads, 23 with 256).
 template <bool NORM>
 static void launch_rows_int8(const RowsI8Args &a, hipStream_t s) {
 #define QTTS_ROWS_I8(W, R, CH, WHEN) if (a.K <= W * 64 * 8 * CH && (WHEN)) { \
@@ -496,7 +496,7 @@ union I8Frag { uint4 u; int4_t v; };
 // k-steps straight from memory to registers; the waves' sums meet in LDS.  U k-steps are requested at a time, the next U
 // before the current are multiplied.  Every weight byte is used 16 TM times at most, so what bounds it is weights coming in:
 // the launch and one latency (1 row x 4096 x 2048: 3.8 us), then the 40-60 GB/s a CU takes of row-major activations and
-// weights together (16 x 2048 x 6144 with residual 7.5 us; SwiGLU 8 x 6144 x 2048 6.7 us, 3.8 TB/s).  Sixteen waves a
+// weights together (16 x 2048 x 6144 with residual 7.6 us; SwiGLU 8 x 6144 x 2048 6.9 us, 3.6 TB/s).  Sixteen waves a
 // workgroup, or the epilogue's scales requested in front of the loop, are no faster.
 template <int TM, int TN, int NW, int U, bool SWIGLU>
 __global__ __launch_bounds__(NW * 64) void linear_int8_split_kernel(LinI8Args a) {
@@ -631,10 +631,10 @@ __device__ __forceinline__ uint32_t lds_address(const void *p) {
 // rows x 64 columns or 8 x 128) stay row-major, the 16-byte chunk c of row r at place c ^ swizzle(r), so that the 16 rows a
 // fragment read touches lie in 16 different places modulo 256 bytes.
 // Small tiles are bound by what comes in: 64 x 64 takes 0.29 us per 128 columns, 0.23 of them for the requests alone (16 KB,
-// 70 GB/s a CU; rows that all lie in L2 would come at 130) and 0.18 for LDS reads and products alone (200 x 4096 x 2048 8.1 us,
+// 70 GB/s a CU; rows that all lie in L2 would come at 117) and 0.18 for LDS reads and products alone (200 x 4096 x 2048 7.8 us,
 // 200 x 2048 x 6144 in 32 x 64 tiles above 13 us).  More stages, eight waves, fragments read a step ahead, padded rows and a
 // start along K that differs between workgroups change nothing or cost 2-9 %.  The largest tile is bound by the matrix units' power: 16384 x 2048 x
-// 6144 in 168-178 us, 2.3-2.4 POPS (the library's product 175-179), at 1.93 GHz - with zeros for data 136 us.  The 32 x 32 x 32
+// 6144 in 171-187 us, 2.2-2.4 POPS (the library's product 175-179), at 1.93 GHz - with zeros for data 136 us.  The 32 x 32 x 32
 // instruction, more stages, and fragments read a step ahead into registers are not faster there (186, 168 and 168 us where
 // this form took 168); without the turns of the two waves of a SIMD (ALT) it takes 183.
 template <int KS>
@@ -943,11 +943,11 @@ __global__ __launch_bounds__(WM * WN * 64) void linear_int8_tile_kernel(LinI8Arg
 // launch's is that times the workgroups a CU gets, on top of what the launch itself takes:
 //   us = launch + (fixed + step * ceil(K / 64)) * load,   load = max(1, r + 3/4 (ceil(r) - r)),  r = workgroups / 256
 // but no less than the weights take from memory at 6 TB/s, times ceil(r) / r for the CUs that idle at the end or throughout
-// (2.4 at most: that is what a CU takes alone; SwiGLU 8 x 6144 x 2048 7.4 us in the form chosen without this, 6.8 with it).  The
+// (2.4 at most: that is what a CU takes alone; SwiGLU 8 x 6144 x 2048 7.5 us in the form chosen without this, 6.9 with it).  The
 // table is fitted to the times of every form over 1-8192 rows and nine N x K from 1024 x 1024 to 8192 x 512 (cold weights, in
-// a graph).  The form with the smallest estimate is taken: 1 % slower on average than the fastest form of each shape, 2 % over
-// 102 others that the fit had not seen (60 drawn at random, 42 with few columns), at most 16 %.  Some of them (us of the forms
-// in the table's order, '-' far off):
+// a graph).  The form with the smallest estimate is taken.  Over 100 shapes drawn at random it is 3.6 % slower on average than the
+// fastest form, by more than 5 % in 22 and by 30-36 % in five: many rows or columns and K below 260, where the fixed parts decide.
+// Some shapes (us of the forms in the table's order, '-' far off):
 //   1 x 4096 x 2048 (plain)       4.0  3.9  4.1  4.7  5.4  4.0  7.7   -    -    -    -
 //   8 x 2048 x 6144 (plain)       7.6  6.2  8.0  8.1   12  5.6   17   -    -    -    -
 //   64 x 2048 x 6144 (plain)       11   11  8.8   12   16   20   17   -    -    -    -

@@ -2,7 +2,9 @@
   python tools/microbench.py launch     # per-launch cost of trivial kernels, eager vs graph
   python tools/microbench.py linear     # skinny-GEMM sweep at the model's shapes
 """
+import math
 import os
+import random
 import sys
 import time
 
@@ -678,53 +680,83 @@ def prefill():
         print(f"prefill {plen:4d} tokens: " + " ".join(f"{v:.2f}" for v in ts) + " ms", flush=True)
 
 
+def graph_us(fn, n=24):
+    """Microseconds per call of fn(0), fn(1), ... fn(n - 1) inside a graph."""
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        fn(0)
+        g = hip.Graph.capture(lambda: [fn(i) for i in range(n)])
+    return timed(lambda: g.launch(), n)
+
+
+def rand_int8(*shape):
+    return torch.randint(-127, 128, shape, device=dev, dtype=torch.int8)
+
+
+def int8_product(what, M, N, K):
+    """A call of the product, weights cold (buffers of 600 MB in turn): "linear", "linear+res" or "swiglu"."""
+    two = what == "swiglu"
+    nbuf = max(1, min(60, int(600e6 // (N * K * (1 + two)))))
+    x = hip.int8_rows(M, K, dev)
+    x.copy_(rand_int8(M, K))
+    xs, ws = torch.rand(M, device=dev), torch.rand(N, device=dev) * 1e-4
+    wp = [hip.pack_gate_up_int8(rand_int8(N, K), rand_int8(N, K)) if two else hip.pack_weight_int8(rand_int8(N, K)) for _ in range(nbuf)]
+    out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+    res = torch.randn(M, N, device=dev).bfloat16() if what == "linear+res" else None
+
+    def run(i):
+        if two:
+            hip.linear_swiglu_int8(x, xs, wp[i % nbuf], ws, ws, N, out=out)
+        else:
+            hip.linear_int8(x, xs, wp[i % nbuf], ws, N, residual=res, out=out)
+
+    return run
+
+
 def int8():
     """The 8-bit operators inside a graph, weights cold: a product in the form the library chooses and in each of the
-    others, rows with a scale each, and the MLP block of them."""
-    R = 24
-    rnd = lambda *shape: torch.randint(-127, 128, shape, device=dev, dtype=torch.int8)   # noqa: E731
-
-    def graph_us(fn, n=R):
-        s = torch.cuda.Stream()
-        with torch.cuda.stream(s):
-            fn(0)
-            g = hip.Graph.capture(lambda: [fn(i) for i in range(n)])
-        return timed(lambda: g.launch(), n)
-
-    for what, M, N, K in (("linear", 1, 4096, 2048), ("linear", 8, 2048, 6144), ("linear+res", 16, 2048, 6144), ("linear", 200, 4096, 2048),
-                          ("linear+res", 777, 1000, 1111), ("linear+res", 16384, 2048, 6144), ("swiglu", 8, 6144, 2048),
-                          ("swiglu", 200, 6144, 2048), ("swiglu", 8192, 6144, 2048)):
-        two = what == "swiglu"
-        nbuf = max(1, min(60, int(600e6 // (N * K * (1 + two)))))
-        x = hip.int8_rows(M, K, dev)
-        x.copy_(rnd(M, K))
-        xs, ws = torch.rand(M, device=dev), torch.rand(N, device=dev) * 1e-4
-        wp = [hip.pack_gate_up_int8(rnd(N, K), rnd(N, K)) if two else hip.pack_weight_int8(rnd(N, K)) for _ in range(nbuf)]
-        out = torch.empty(M, N, device=dev, dtype=torch.bfloat16)
-        res = torch.randn(M, N, device=dev).bfloat16() if what == "linear+res" else None
-
-        def run(i):
-            if two:
-                hip.linear_swiglu_int8(x, xs, wp[i % nbuf], ws, ws, N, out=out)
-            else:
-                hip.linear_int8(x, xs, wp[i % nbuf], ws, N, residual=res, out=out)
-
-        n = R if M < 1000 else 4
+    others, rows with a scale each (cold too where eight buffers of them pass the last-level cache), products beside the
+    bf16 and fp8 ones, and the MLP block."""
+    for what, M, N, K in (("linear", 1, 4096, 2048), ("linear", 8, 2048, 6144), ("linear+res", 16, 2048, 6144), ("linear+res", 64, 2048, 6144),
+                          ("linear", 200, 4096, 2048), ("linear+res", 200, 2048, 6144), ("linear+res", 512, 2048, 6144),
+                          ("linear+res", 1024, 2048, 6144), ("linear+res", 777, 1000, 1111), ("linear+res", 16384, 2048, 6144),
+                          ("swiglu", 8, 6144, 2048), ("swiglu", 200, 6144, 2048), ("swiglu", 8192, 6144, 2048)):
+        run, n = int8_product(what, M, N, K), 24 if M < 1000 else 4
         us = []
         for form in (*range(11), -1):                    # -1: the library's choice
             hip.lib.qtts_tune_int8(form)
             us.append(graph_us(run, n))
-        ops = 2 * M * N * K * (1 + two)
+        ops = 2 * M * N * K * (1 + (what == "swiglu"))
         print(f"{what:10s} {M:5d} x {N} x {K}: {us[-1]:6.1f} us {ops / us[-1] / 1e6:5.0f} TOPS   forms " + " ".join(f"{u:.1f}" for u in us[:-1]),
               flush=True)
-    for what, M, K in (("rmsnorm", 8, 2048), ("rmsnorm", 16384, 2048), ("quantize", 333, 1111), ("quantize", 8192, 6144)):
-        x, d, w = (torch.randn(*s, device=dev).bfloat16() for s in ((M, K), (M, K), (K,)))
-        h, q, s = torch.empty_like(x), hip.int8_rows(M, K, dev), torch.empty(M, device=dev)
+    for what, M, K in (("rmsnorm", 8, 2048), ("rmsnorm", 16384, 2048), ("rmsnorm", 8192, 6144), ("rmsnorm", 16384, 256), ("rmsnorm", 300, 40000),
+                       ("quantize", 333, 1111), ("quantize", 8192, 6144), ("quantize", 300, 40000)):
+        xs, ds = ([torch.randn(M, K, device=dev).bfloat16() for _ in range(8)] for _ in range(2))
+        w, h, q, s = torch.randn(K, device=dev).bfloat16(), torch.empty_like(xs[0]), hip.int8_rows(M, K, dev), torch.empty(M, device=dev)
         if what == "rmsnorm":
-            us, by = graph_us(lambda i: hip.rmsnorm_int8(x, w, delta=d, sum_out=h, out=q, scales=s)), 7 * M * K
+            us, by = graph_us(lambda i: hip.rmsnorm_int8(xs[i % 8], w, delta=ds[i % 8], sum_out=h, out=q, scales=s)), 7 * M * K
         else:
-            us, by = graph_us(lambda i: hip.quantize_int8(x, out=q, scales=s)), 3 * M * K
+            us, by = graph_us(lambda i: hip.quantize_int8(xs[i % 8], out=q, scales=s)), 3 * M * K
         print(f"{what:10s} {M:5d} x {K}: {us:6.1f} us {by / us / 1e6:5.2f} TB/s", flush=True)
+        del xs, ds, h, q
+    for what, N, K in (("gate/up", 6144, 2048), ("down", 2048, 6144)):
+        two = what == "gate/up"
+        bf = lambda n: [(torch.randn(N, K, device=dev) * 0.02).bfloat16() for _ in range(n)]    # noqa: E731
+        nbuf = 12
+        if two:
+            w16, w8 = [hip.pack_gate_up(a, a) for a in bf(nbuf)], [hip.pack_gate_up_fp8(a, a) for a in bf(nbuf)]
+        else:
+            w16, w8 = [hip.pack_weight(a) for a in bf(nbuf)], [hip.pack_weight_fp8(a) for a in bf(nbuf)]
+        for M in (1, 8, 64, 200, 1024):
+            x, out = torch.randn(M, K, device=dev).bfloat16(), torch.empty(M, N, device=dev, dtype=torch.bfloat16)
+            if two:
+                u16 = graph_us(lambda i: hip.linear_swiglu(x, w16[i % nbuf], N, out=out))
+                u8 = graph_us(lambda i: hip.linear_swiglu_fp8(x, *w8[i % nbuf], N, out=out))
+            else:
+                u16 = graph_us(lambda i: hip.linear_ws(x, w16[i % nbuf], N, out=out))
+                u8 = graph_us(lambda i: hip.linear_fp8(x, *w8[i % nbuf], N, out=out))
+            ui = graph_us(int8_product("swiglu" if two else "linear", M, N, K))
+            print(f"{what:8s} {M:5d} x {N} x {K}: bf16 {u16:6.1f} us  fp8 weights {u8:6.1f} us  int8 {ui:6.1f} us", flush=True)
     H, I = 2048, 6144
     q = lambda n, k: hip.quantize_int8((torch.randn(n, k, device=dev) * k ** -0.5).bfloat16())   # noqa: E731
     nbuf = 16
@@ -748,6 +780,28 @@ def int8():
         print(f"MLP block  {M:5d} rows: {graph_us(block, nbuf):6.1f} us", flush=True)
 
 
+def int8forms():
+    """The form the library chooses for an int8 product against the fastest of the eleven, over shapes drawn at random."""
+    rng = random.Random(7)
+    size = lambda low, high: int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))   # noqa: E731
+    worse = []
+    while len(worse) < 100:
+        what, M, N, K = rng.choice(("linear", "swiglu")), size(1, 8192), size(64, 8192), size(64, 8192)
+        ops = 2 * M * N * K * (1 + (what == "swiglu"))
+        if ops > 4e11:
+            continue
+        run, n, us = int8_product(what, M, N, K), 24 if ops < 1e10 else 4, []
+        chosen = hip.lib.qtts_linear_int8_form(M, N, K, int(what == "swiglu"))
+        for form in range(11):
+            hip.lib.qtts_tune_int8(form)
+            us.append(graph_us(run, n))
+        hip.lib.qtts_tune_int8(-1)
+        worse.append(us[chosen] / min(us) - 1)
+        print(f"{what:6s} {M:5d} x {N:5d} x {K:5d}: form {chosen:2d} {us[chosen]:6.1f} us, {100 * worse[-1]:4.1f} % over form {us.index(min(us)):2d}", flush=True)
+    print(f"{len(worse)} shapes: {100 * sum(worse) / len(worse):.1f} % over the fastest form on average, {100 * max(worse):.0f} % at most, "
+          f"{sum(w > 0.05 for w in worse)} by more than 5 %", flush=True)
+
+
 if __name__ == "__main__":
     _tuning.apply_env_flags()
-    {"prefill": prefill, "prefill_batch": prefill_batch, "decode_eager": decode_eager, "rows": rows, "rowsn": rowsn, "attn": attn, "attntrace": attntrace, "rowtrace": rowtrace, "launch": launch, "linear": linear, "linear2": linear2, "frame": frame, "dominant": dominant, "lat": lat, "mall": mall, "gridbar": gridbar, "trace": trace, "int8": int8}[sys.argv[1]]()
+    {"prefill": prefill, "prefill_batch": prefill_batch, "decode_eager": decode_eager, "rows": rows, "rowsn": rowsn, "attn": attn, "attntrace": attntrace, "rowtrace": rowtrace, "launch": launch, "linear": linear, "linear2": linear2, "frame": frame, "dominant": dominant, "lat": lat, "mall": mall, "gridbar": gridbar, "trace": trace, "int8": int8, "int8forms": int8forms}[sys.argv[1]]()
